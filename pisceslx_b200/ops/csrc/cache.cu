@@ -1,0 +1,276 @@
+// A paged cache in 8 bits: keys and values become e4m3 codes with one power of two for each token and head as they are written,
+// and are read back.  Attention over such pages, or over pages in bf16: cache_attn.cuh.
+//
+// A row x of d numbers (one head of one token) is held as code_i 2^E: E is the smallest exponent at which the largest |x_i| does
+// not pass 448, e4m3's largest number, and code_i = x_i 2^-E to the nearest e4m3 number (ties to even).  The codes are floating
+// point, so a finer factor than a power of two would not make them more exact; a power of two makes the product x_i 2^-E exact,
+// the row's byte an exponent, and the value read back a bf16 number without rounding.  A row with a number that is not finite gets
+// the byte 255 and is read as NaN throughout.
+#include <cuda_fp8.h>
+
+#include "cache_attn.cuh"
+#include "cache_ops.h"
+#include "chain.cuh"
+#include "sm100.cuh"
+
+namespace yv {
+namespace {
+
+constexpr int kRowsThreads = 256;
+
+// One group of d / 8 lanes per row: 16 bytes in, 8 bytes of codes out, a byte by the first lane.
+template <int D, bool CHAIN>
+__global__ void __launch_bounds__(kRowsThreads) cache_write_fp8_kernel(const CacheRowsArgs a) {
+  constexpr int kLanes = D / 8;
+  chain_start<CHAIN>();
+  const int64_t at = (static_cast<int64_t>(blockIdx.x) * kRowsThreads + threadIdx.x) / kLanes;
+  const int lane = threadIdx.x % kLanes;
+  const int per = 2 * a.hk;
+  const int64_t t = at / per;
+  if (t >= a.tokens) return;                                   // whole groups of lanes leave together
+  const int r = static_cast<int>(at - t * per);
+  const bool val = r >= a.hk;
+  const int h = val ? r - a.hk : r;
+  const int slot = a.slots[t];
+  if (slot < 0) return;
+  if (slot >= a.num_slots) {
+    if (lane == 0 && a.status != nullptr) atomicOr(a.status, kStatusIndexOutOfRange);
+    return;
+  }
+  const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(val ? a.v : a.k) + t * (val ? a.v_ld : a.k_ld) +
+                             static_cast<int64_t>(h) * D + lane * 8;
+  const uint4 x = *reinterpret_cast<const uint4*>(src);
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  // magnitudes of bf16 numbers are ordered as integers; what is not finite is above all others
+  uint32_t m2 = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m2 = __vmaxu2(m2, w[i] & 0x7FFF7FFFu);
+  uint32_t top = max(m2 & 0xFFFFu, m2 >> 16);
+  const unsigned mask = ((1u << kLanes) - 1u) << (threadIdx.x & 31 & ~(kLanes - 1));      // a group leaves as one
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(mask, top, o));
+  // top = 1.f 2^(X - 127) against 448 = 1.75 2^8
+  const bool finite = top < 0x7F80u;
+  const int byte = finite ? max(0, static_cast<int>(top >> 7) - 8 + ((top & 0x7Fu) > 0x60u ? 1 : 0)) : 255;
+  const float inv = __int_as_float((254 - (finite ? byte : 127)) << 23);          // 2^-E
+  uint32_t c[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint32_t both = 0;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t p = w[2 * i + j];
+      const float2 f = make_float2(__uint_as_float(p << 16) * inv, __uint_as_float(p & 0xFFFF0000u) * inv);
+      both |= static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3)) << (16 * j);
+    }
+    c[i] = finite ? both : 0x7F7F7F7Fu;
+  }
+  uint8_t* dst = static_cast<uint8_t*>(val ? a.v_codes : a.k_codes) + (static_cast<int64_t>(slot) * a.hk + h) * D + lane * 8;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(c[0], c[1]);
+  if (lane == 0) {
+    const int page = slot / a.block;
+    static_cast<uint8_t*>(val ? a.v_scale : a.k_scale)[(static_cast<int64_t>(page) * a.hk + h) * a.block + slot - page * a.block] =
+        static_cast<uint8_t>(byte);
+  }
+}
+
+// 2^(byte - 127) in fp32
+__device__ __forceinline__ float scale_of(uint32_t byte) {
+  return __uint_as_float(byte == 255u ? 0x7FC00000u : byte == 0u ? 0x00400000u : byte << 23);
+}
+
+template <int D>
+__global__ void __launch_bounds__(kRowsThreads) cache_read_fp8_kernel(const CacheRowsArgs a) {
+  constexpr int kLanes = D / 16;
+  const int64_t at = (static_cast<int64_t>(blockIdx.x) * kRowsThreads + threadIdx.x) / kLanes;
+  const int lane = threadIdx.x % kLanes;
+  const int per = 2 * a.hk;
+  const int64_t t = at / per;
+  if (t >= a.tokens) return;
+  const int r = static_cast<int>(at - t * per);
+  const bool val = r >= a.hk;
+  const int h = val ? r - a.hk : r;
+  const int slot = a.slots[t];
+  uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (slot >= a.num_slots) {
+    if (lane == 0 && a.status != nullptr) atomicOr(a.status, kStatusIndexOutOfRange);
+  } else if (slot >= 0) {
+    const uint4 c = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(val ? a.v_codes : a.k_codes) +
+                                                    (static_cast<int64_t>(slot) * a.hk + h) * D + lane * 16);
+    const int page = slot / a.block;
+    const float s = scale_of(static_cast<const uint8_t*>(
+        val ? a.v_scale : a.k_scale)[(static_cast<int64_t>(page) * a.hk + h) * a.block + slot - page * a.block]);
+    const uint32_t codes[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const __half2_raw two = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(codes[i >> 1] >> (16 * (i & 1))), __NV_E4M3);
+      const float2 f = __half22float2(__half2(two));
+      w[i] = pack_bf16(f.x * s, f.y * s);
+    }
+  }
+  __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(val ? a.vo : a.ko) + (t * a.hk + h) * D + lane * 16;
+  reinterpret_cast<uint4*>(dst)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  reinterpret_cast<uint4*>(dst)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+}
+
+bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+int rows_grid(const CacheRowsArgs& a, int lanes, unsigned* grid) {
+  if (a.hk <= 0 || (a.d != 64 && a.d != 128) || a.block <= 0 || a.num_slots < 0 || a.num_slots >= (1ll << 31)) return -1;
+  const int64_t blocks = (a.tokens * 2 * a.hk * lanes + kRowsThreads - 1) / kRowsThreads;
+  if (blocks > 0x7FFFFFFFll) return -2;
+  *grid = static_cast<unsigned>(blocks);
+  return 0;
+}
+
+}  // namespace
+
+int launch_cache_write_fp8(const CacheRowsArgs& in, cudaStream_t stream) {
+  CacheRowsArgs a = in;
+  if (a.tokens <= 0) return 0;
+  if (a.tokens == 1) a.k_ld = a.v_ld = 0;                      // a single row has no pitch
+  unsigned grid = 0;
+  const int r = rows_grid(a, a.d / 8, &grid);
+  if (r != 0) return r;
+  if (((a.k_ld | a.v_ld) & 7) != 0 || !al16(a.k) || !al16(a.v) || !al16(a.k_codes) || !al16(a.v_codes)) return -3;
+  const bool chain = grid <= kChainBlocks;
+  if (a.d == 128)
+    return launch_chained_if(chain, cache_write_fp8_kernel<128, true>, cache_write_fp8_kernel<128, false>, dim3(grid), dim3(kRowsThreads), 0, stream, a);
+  return launch_chained_if(chain, cache_write_fp8_kernel<64, true>, cache_write_fp8_kernel<64, false>, dim3(grid), dim3(kRowsThreads), 0, stream, a);
+}
+
+int launch_cache_read_fp8(const CacheRowsArgs& a, cudaStream_t stream) {
+  if (a.tokens <= 0) return 0;
+  unsigned grid = 0;
+  const int r = rows_grid(a, a.d / 16, &grid);
+  if (r != 0) return r;
+  if (!al16(a.ko) || !al16(a.vo) || !al16(a.k_codes) || !al16(a.v_codes)) return -3;
+  (a.d == 128 ? cache_read_fp8_kernel<128> : cache_read_fp8_kernel<64>)<<<grid, kRowsThreads, 0, stream>>>(a);
+  return static_cast<int>(cudaGetLastError());
+}
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+int sm_count() {
+  static PerDeviceInt count;
+  if (!count.cur()) {
+    int dev = 0, n = 0;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    count.cur() = n > 0 ? n : 148;
+  }
+  return count.cur();
+}
+
+// Tokens of a query tile, whether blocks have two tiles, and the items of one key range.
+struct CacheGrid {
+  int per_tile, two;
+  int64_t items;
+};
+CacheGrid cache_grid(const CacheAttnArgs& a) {
+  CacheGrid g;
+  g.per_tile = kCaTile / (a.hq / a.hk);
+  const int64_t heads = static_cast<int64_t>(a.hk) * a.batch, tiles = (a.max_q + g.per_tile - 1) / g.per_tile;
+  g.two = tiles * heads > sm_count();
+  g.items = (g.two ? (tiles + 1) / 2 : tiles) * heads;
+  return g;
+}
+
+int check(const CacheAttnArgs& a) {
+  if (a.d != 64 && a.d != 128) return -1;
+  if (a.hk <= 0 || a.hq <= 0 || a.hq % a.hk != 0 || a.hq / a.hk > kCaTile) return -2;
+  if (a.block <= 0 || a.block % 16 != 0 || a.table_width <= 0 || a.num_blocks <= 0 ||
+      static_cast<int64_t>(a.num_blocks) * a.block >= (1ll << 31) || static_cast<int64_t>(a.table_width) * a.block >= (1ll << 30)) return -3;
+  if (a.window < 0 || a.first < 0 || !(a.scale > 0.f) || a.max_q <= 0) return -4;
+  if (!al16(a.q) || !al16(a.o) || !al16(a.k) || !al16(a.v) || ((a.q_ld | a.o_ld) & 7) != 0) return -5;
+  return 0;
+}
+
+template <int D, bool F8>
+int run_cache_attn(const CacheAttnParams& p, unsigned grid, cudaStream_t stream) {
+  using S = CacheAttn<D, F8>;
+  static PerDeviceInt configured;
+  if (!configured.cur()) {
+    const cudaError_t e = cudaFuncSetAttribute(cache_attn_kernel<D, F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kTotal);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    configured.cur() = 1;
+  }
+  cache_attn_kernel<D, F8><<<grid, S::kThreads, S::kTotal, stream>>>(p);
+  return static_cast<int>(cudaGetLastError());
+}
+
+int page_map(CUtensorMap* m, const CacheAttnArgs& a, const void* pages, int box) {
+  return make_tmap_3d(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, pages, static_cast<uint64_t>(a.d), static_cast<uint64_t>(a.hk),
+                      static_cast<uint64_t>(a.num_blocks) * a.block, static_cast<uint64_t>(a.d) * 2,
+                      static_cast<uint64_t>(a.hk) * a.d * 2, 64, 1, static_cast<uint32_t>(box));
+}
+
+}  // namespace
+
+int cache_attn_splits(const CacheAttnArgs& a) {
+  if (check(a) != 0 || a.batch <= 0) return 1;
+  const CacheGrid g = cache_grid(a);
+  const int sms = sm_count();
+  int64_t keys = static_cast<int64_t>(a.table_width) * a.block;
+  if (a.window > 0) keys = keys < a.window + a.first + a.max_q ? keys : a.window + a.first + a.max_q;
+  // steps of an item: key tiles of a block of two query tiles, pairs of key tiles of a lone one
+  const double steps = static_cast<double>((keys + kCaTile - 1) / kCaTile) / (g.two ? 1 : 2);
+  const int64_t room = (int64_t(256) << 20) / (a.total_q * a.hq * a.d * 4 + 1);              // ranges that the scratch has room for
+  int best = 1;
+  double least = 0;
+  for (int s = 1; s <= 32 && (s == 1 || (s <= 2 * steps && s <= room)); ++s) {
+    const double cost = static_cast<double>((g.items * s + sms - 1) / sms) * (steps / s + 2) + (s > 1 ? 3 + 0.1 * s : 0);
+    if (s == 1 || cost < least) { best = s; least = cost; }
+  }
+  return best;
+}
+
+int launch_cache_attn(const CacheAttnArgs& a, cudaStream_t stream) {
+  if (a.total_q <= 0 || a.batch <= 0) return 0;
+  int r = check(a);
+  if (r != 0) return r;
+  const bool f8 = a.k_scale != nullptr;
+  if (a.splits < 1 || (a.splits > 1 && (a.partial_o == nullptr || a.partial_ml == nullptr))) return -6;
+  const CacheGrid g = cache_grid(a);
+  CacheAttnParams p = {};
+  p.group = a.hq / a.hk; p.per_tile = g.per_tile;
+  r = make_tmap_3d(&p.tma_q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.q, static_cast<uint64_t>(a.d), static_cast<uint64_t>(a.hq),
+                   static_cast<uint64_t>(a.total_q), static_cast<uint64_t>(a.d) * 2, static_cast<uint64_t>(a.q_ld) * 2, 64,
+                   static_cast<uint32_t>(p.group), static_cast<uint32_t>(p.per_tile));
+  if (r != 0) return -10 + r;
+  // rows of one copy: a power of two that divides a page
+  p.box = 16;
+  while (p.box < kCaTile && a.block % (2 * p.box) == 0) p.box *= 2;
+  if (f8) {
+    p.k8 = static_cast<const uint8_t*>(a.k); p.v8 = static_cast<const uint8_t*>(a.v);
+    p.ks = static_cast<const uint8_t*>(a.k_scale); p.vs = static_cast<const uint8_t*>(a.v_scale);
+  } else {
+    r = page_map(&p.tma_k, a, a.k, p.box);
+    if (r != 0) return -20 + r;
+    r = page_map(&p.tma_v, a, a.v, p.box);
+    if (r != 0) return -30 + r;
+  }
+  p.o = static_cast<__nv_bfloat16*>(a.o); p.o_ld = a.o_ld;
+  p.po = a.partial_o; p.pml = a.partial_ml;
+  p.cu_q = a.cu_q; p.table = a.table; p.lens = a.lens;
+  p.total_q = a.total_q;
+  p.hq = a.hq; p.hk = a.hk; p.batch = a.batch; p.max_q = a.max_q;
+  p.block = a.block; p.num_blocks = a.num_blocks; p.table_width = a.table_width;
+  p.window = a.window; p.first = a.window > 0 ? a.first : 0;
+  p.two = g.two; p.splits = a.splits; p.items = g.items * a.splits;
+  p.zero_rest = a.zero_rest ? 1 : 0;
+  p.scale_log2 = a.scale * kLog2e;
+  p.status = a.status;
+  const int sms = sm_count();
+  const unsigned grid = static_cast<unsigned>(p.items < sms ? p.items : sms);
+  if (a.d == 128) r = f8 ? run_cache_attn<128, true>(p, grid, stream) : run_cache_attn<128, false>(p, grid, stream);
+  else r = f8 ? run_cache_attn<64, true>(p, grid, stream) : run_cache_attn<64, false>(p, grid, stream);
+  if (r != 0 || a.splits == 1) return r;
+  const unsigned rows = static_cast<unsigned>((a.total_q * a.hq + 3) / 4);
+  (a.d == 128 ? cache_attn_merge_kernel<128> : cache_attn_merge_kernel<64>)<<<rows, 128, 0, stream>>>(p);
+  return static_cast<int>(cudaGetLastError());
+}
+
+}  // namespace yv

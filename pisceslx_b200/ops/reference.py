@@ -278,6 +278,84 @@ def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     return torch.stack(outs).to(q.dtype)
 
 
+def fp8_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows x [..., d] -> (e4m3 codes, exponent bytes [...]): code * 2 ** (byte - 127), see ``ops.cache``."""
+    xf = x.float()
+    finite = torch.isfinite(xf).all(-1)
+    xf = torch.where(finite.unsqueeze(-1), xf, torch.zeros_like(xf))
+    top = xf.abs().amax(-1) if x.shape[-1] else xf.sum(-1)
+    m, e = torch.frexp(top)                                  # top = m 2^e with m in [1/2, 1); 448 = 0.875 * 2^9
+    e = torch.where(top > 0, e - 9 + (m > 0.875).int(), torch.full_like(e, -127)).clamp_min(-127)
+    codes = torch.ldexp(xf.double(), -e.unsqueeze(-1)).float().to(torch.float8_e4m3fn)
+    codes = torch.where(finite.unsqueeze(-1), codes.view(torch.uint8), torch.full_like(codes.view(torch.uint8), 0x7F))
+    return codes.view(torch.float8_e4m3fn), torch.where(finite, e + 127, torch.full_like(e, 255)).to(torch.uint8)
+
+
+def _fp8_values(codes: torch.Tensor, byte: torch.Tensor) -> torch.Tensor:
+    x = torch.ldexp(codes.float().double(), (byte.int() - 127).unsqueeze(-1)).float()
+    return torch.where((byte == 255).unsqueeze(-1), torch.full_like(x, float("nan")), x)
+
+
+def _cache_slots(slot_map: torch.Tensor, block: int, blocks: int) -> Tuple[torch.Tensor, torch.Tensor]:
+    if slot_map.numel() and int(slot_map.max()) >= block * blocks:
+        raise IndexError(f"slot {int(slot_map.max())} of a pool of {block * blocks}")
+    at = slot_map.clamp_min(0).long()
+    return at // block, at % block
+
+
+def kv_cache_write_fp8(k, v, k_cache, v_cache, k_scale, v_scale, slot_map) -> None:
+    blocks, block, hk, d = k_cache.shape
+    keep = slot_map >= 0
+    page, at = _cache_slots(slot_map[keep], block, blocks)
+    for x, codes, scale in ((k, k_cache, k_scale), (v, v_cache, v_scale)):
+        c, e = fp8_rows(x[keep].reshape(-1, hk, d))
+        codes.view(torch.uint8)[page, at] = c.view(torch.uint8)
+        scale[page, :, at] = e
+
+
+def kv_cache_read_fp8(k_cache, v_cache, k_scale, v_scale, slot_map) -> Tuple[torch.Tensor, torch.Tensor]:
+    blocks, block, hk, d = k_cache.shape
+    page, at = _cache_slots(slot_map, block, blocks)
+    gone = (slot_map < 0).view(-1, 1, 1)
+    take = lambda c, e: _fp8_values(c.view(torch.uint8)[page, at].view(torch.float8_e4m3fn), e[page, :, at]).masked_fill(gone, 0.0)
+    return tuple(take(c, e).reshape(-1, hk * d).to(torch.bfloat16) for c, e in ((k_cache, k_scale), (v_cache, v_scale)))
+
+
+def cache_attention(q, k_cache, v_cache, block_table, seq_lens, cu_q, scale, window, first_tokens, k_scale, v_scale, out):
+    """Causal attention over pages with an optional window and first tokens that stay visible; see ``ops.cache``."""
+    T, hq, d = q.shape
+    blocks, block, hk = k_cache.shape[:3]
+    cuts = cu_q.tolist() if cu_q is not None else list(range(block_table.shape[0] + 1))
+    o = torch.zeros_like(q) if out is None else out
+    for b, n in enumerate(seq_lens.tolist()):
+        new = cuts[b + 1] - cuts[b]
+        rows = slice(cuts[b], cuts[b + 1])
+        pos = torch.arange(n - new, n).view(-1, 1)
+        key = torch.arange(n).view(1, -1)
+        ok = key <= pos
+        if window is not None:
+            ok &= (key > pos - window) | (key < first_tokens)
+        o[rows] = 0
+        seen = ok.any(0).nonzero().flatten()
+        if new == 0 or seen.numel() == 0:
+            continue
+        page = block_table[b, seen // block].long()
+        if int(page.min()) < 0 or int(page.max()) >= blocks:
+            raise IndexError(f"sequence {b}: a page outside the pool of {blocks}")
+        at = seen % block
+        if k_scale is None:
+            kk, vv = k_cache[page, at].float(), v_cache[page, at].float()
+        else:
+            kk, vv = (_fp8_values(c.view(torch.uint8)[page, at].view(torch.float8_e4m3fn), e[page, :, at])
+                      for c, e in ((k_cache, k_scale), (v_cache, v_scale)))
+        mask = ok[:, seen]
+        sc = torch.einsum("mhgd,nhd->hgmn", q[rows].float().view(new, hk, hq // hk, d), kk) * scale
+        sc = sc.masked_fill(~mask, float("-inf"))
+        w = torch.softmax(sc, -1).masked_fill(~mask.any(1).view(1, 1, -1, 1), 0.0)
+        o[rows] = torch.einsum("hgmn,nhd->mhgd", w, vv).reshape(new, hq, d).to(q.dtype)
+    return o
+
+
 # --------------------------------------------------------------------------------------------------
 # loss
 # --------------------------------------------------------------------------------------------------
