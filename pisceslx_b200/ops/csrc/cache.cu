@@ -9,8 +9,8 @@
 #include <cuda_fp8.h>
 
 #include "cache_attn.cuh"
+#include "cache_few.cuh"
 #include "cache_ops.h"
-#include "chain.cuh"
 #include "sm100.cuh"
 
 namespace yv {
@@ -152,6 +152,7 @@ int launch_cache_read_fp8(const CacheRowsArgs& a, cudaStream_t stream) {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kFewMost = 128;
 
 int sm_count() {
   static PerDeviceInt count;
@@ -173,7 +174,7 @@ CacheGrid cache_grid(const CacheAttnArgs& a) {
   CacheGrid g;
   g.per_tile = kCaTile / (a.hq / a.hk);
   const int64_t heads = static_cast<int64_t>(a.hk) * a.batch, tiles = (a.max_q + g.per_tile - 1) / g.per_tile;
-  g.two = tiles * heads > sm_count();
+  g.two = tiles > 1;
   g.items = (g.two ? (tiles + 1) / 2 : tiles) * heads;
   return g;
 }
@@ -188,22 +189,29 @@ int check(const CacheAttnArgs& a) {
   return 0;
 }
 
-template <int D, bool F8>
+template <int D>
 int run_cache_attn(const CacheAttnParams& p, unsigned grid, cudaStream_t stream) {
-  using S = CacheAttn<D, F8>;
+  using S = CacheAttn<D>;
   static PerDeviceInt configured;
   if (!configured.cur()) {
-    const cudaError_t e = cudaFuncSetAttribute(cache_attn_kernel<D, F8>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kTotal);
+    const cudaError_t e = cudaFuncSetAttribute(cache_attn_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kTotal);
     if (e != cudaSuccess) return static_cast<int>(e);
     configured.cur() = 1;
   }
-  cache_attn_kernel<D, F8><<<grid, S::kThreads, S::kTotal, stream>>>(p);
+  cache_attn_kernel<D><<<grid, S::kThreads, S::kTotal, stream>>>(p);
   return static_cast<int>(cudaGetLastError());
 }
 
-int page_map(CUtensorMap* m, const CacheAttnArgs& a, const void* pages, int box) {
+// Rows (token, head of a group) a tile of the kernel for few tokens holds, 0 where cache_attn_kernel takes the call.
+int few_rows(const CacheAttnArgs& a) {
+  const int64_t rows = static_cast<int64_t>(a.max_q) * (a.hq / a.hk);
+  if (a.hq / a.hk > 64 || rows > kFewMost) return 0;
+  return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+}
+
+int page_map(CUtensorMap* m, const CacheAttnArgs& a, const void* pages, int64_t slots, int box) {
   return make_tmap_3d(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, pages, static_cast<uint64_t>(a.d), static_cast<uint64_t>(a.hk),
-                      static_cast<uint64_t>(a.num_blocks) * a.block, static_cast<uint64_t>(a.d) * 2,
+                      static_cast<uint64_t>(slots), static_cast<uint64_t>(a.d) * 2,
                       static_cast<uint64_t>(a.hk) * a.d * 2, 64, 1, static_cast<uint32_t>(box));
 }
 
@@ -211,8 +219,13 @@ int page_map(CUtensorMap* m, const CacheAttnArgs& a, const void* pages, int box)
 
 int cache_attn_splits(const CacheAttnArgs& a) {
   if (check(a) != 0 || a.batch <= 0) return 1;
-  const CacheGrid g = cache_grid(a);
-  const int sms = sm_count();
+  CacheGrid g = cache_grid(a);
+  const int sms = sm_count(), few = few_rows(a);
+  if (few != 0) {
+    const int per = few / (a.hq / a.hk);
+    g.two = 1;
+    g.items = static_cast<int64_t>(a.hk) * a.batch * ((a.max_q + per - 1) / per);
+  }
   int64_t keys = static_cast<int64_t>(a.table_width) * a.block;
   if (a.window > 0) keys = keys < a.window + a.first + a.max_q ? keys : a.window + a.first + a.max_q;
   // steps of an item: key tiles of a block of two query tiles, pairs of key tiles of a lone one
@@ -227,31 +240,24 @@ int cache_attn_splits(const CacheAttnArgs& a) {
   return best;
 }
 
-int launch_cache_attn(const CacheAttnArgs& a, cudaStream_t stream) {
-  if (a.total_q <= 0 || a.batch <= 0) return 0;
-  int r = check(a);
-  if (r != 0) return r;
-  const bool f8 = a.k_scale != nullptr;
-  if (a.splits < 1 || (a.splits > 1 && (a.partial_o == nullptr || a.partial_ml == nullptr))) return -6;
-  const CacheGrid g = cache_grid(a);
+int cache_attn_wide_batch(const CacheAttnArgs& a) {
+  if (a.k_scale == nullptr || check(a) != 0 || a.batch <= 0 || few_rows(a) != 0) return 0;
+  // about a gigabyte at a time, one sequence at least
+  const int64_t one = static_cast<int64_t>(a.table_width) * a.block * a.hk * a.d * 4, fit = (int64_t(1) << 30) / one;
+  return static_cast<int>(fit < 1 ? 1 : fit < a.batch ? fit : a.batch);
+}
+
+namespace {
+
+int launch_merge(const CacheAttnParams& p, int d, cudaStream_t stream) {
+  const dim3 grid(static_cast<unsigned>((p.total_q * p.hq + 3) / 4));
+  return launch_chained(d == 128 ? cache_attn_merge_kernel<128> : cache_attn_merge_kernel<64>, grid, dim3(128), 0, stream, 0, p);
+}
+
+// What both kernels read of the sequences.
+CacheAttnParams cache_params(const CacheAttnArgs& a) {
   CacheAttnParams p = {};
-  p.group = a.hq / a.hk; p.per_tile = g.per_tile;
-  r = make_tmap_3d(&p.tma_q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.q, static_cast<uint64_t>(a.d), static_cast<uint64_t>(a.hq),
-                   static_cast<uint64_t>(a.total_q), static_cast<uint64_t>(a.d) * 2, static_cast<uint64_t>(a.q_ld) * 2, 64,
-                   static_cast<uint32_t>(p.group), static_cast<uint32_t>(p.per_tile));
-  if (r != 0) return -10 + r;
-  // rows of one copy: a power of two that divides a page
-  p.box = 16;
-  while (p.box < kCaTile && a.block % (2 * p.box) == 0) p.box *= 2;
-  if (f8) {
-    p.k8 = static_cast<const uint8_t*>(a.k); p.v8 = static_cast<const uint8_t*>(a.v);
-    p.ks = static_cast<const uint8_t*>(a.k_scale); p.vs = static_cast<const uint8_t*>(a.v_scale);
-  } else {
-    r = page_map(&p.tma_k, a, a.k, p.box);
-    if (r != 0) return -20 + r;
-    r = page_map(&p.tma_v, a, a.v, p.box);
-    if (r != 0) return -30 + r;
-  }
+  p.group = a.hq / a.hk;
   p.o = static_cast<__nv_bfloat16*>(a.o); p.o_ld = a.o_ld;
   p.po = a.partial_o; p.pml = a.partial_ml;
   p.cu_q = a.cu_q; p.table = a.table; p.lens = a.lens;
@@ -259,18 +265,128 @@ int launch_cache_attn(const CacheAttnArgs& a, cudaStream_t stream) {
   p.hq = a.hq; p.hk = a.hk; p.batch = a.batch; p.max_q = a.max_q;
   p.block = a.block; p.num_blocks = a.num_blocks; p.table_width = a.table_width;
   p.window = a.window; p.first = a.window > 0 ? a.first : 0;
-  p.two = g.two; p.splits = a.splits; p.items = g.items * a.splits;
+  p.splits = a.splits;
   p.zero_rest = a.zero_rest ? 1 : 0;
   p.scale_log2 = a.scale * kLog2e;
   p.status = a.status;
+  // rows of one copy: a power of two that divides a page
+  p.box = 16;
+  while (p.box < kCaTile && a.block % (2 * p.box) == 0) p.box *= 2;
+  return p;
+}
+
+template <int D, bool F8, int N>
+int run_cache_few(const CacheFewParams& p, unsigned grid, cudaStream_t stream) {
+  using S = CacheFew<D, F8, N>;
+  static PerDeviceInt configured;
+  if (!configured.cur()) {
+    const cudaError_t e = cudaFuncSetAttribute(cache_few_kernel<D, F8, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kTotal);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    configured.cur() = 1;
+  }
+  return launch_chained(cache_few_kernel<D, F8, N>, dim3(grid), dim3(S::kThreads), S::kTotal, stream, 0, p);
+}
+
+template <int D, bool F8>
+int run_cache_few(const CacheFewParams& p, int rows, unsigned grid, cudaStream_t stream) {
+  return rows == 16 ? run_cache_few<D, F8, 16>(p, grid, stream) : rows == 32 ? run_cache_few<D, F8, 32>(p, grid, stream)
+                                                                             : run_cache_few<D, F8, 64>(p, grid, stream);
+}
+
+int code_map(CUtensorMap* m, const CacheAttnArgs& a, const void* codes, int box, CUtensorMapSwizzle swizzle) {
+  return make_tmap_3d(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes, static_cast<uint64_t>(a.d), static_cast<uint64_t>(a.hk),
+                      static_cast<uint64_t>(a.num_blocks) * a.block, static_cast<uint64_t>(a.d), static_cast<uint64_t>(a.hk) * a.d,
+                      static_cast<uint32_t>(a.d), 1, static_cast<uint32_t>(box), swizzle);
+}
+
+int launch_cache_few(const CacheAttnArgs& a, int rows, cudaStream_t stream) {
+  CacheFewParams f = {};
+  f.a = cache_params(a);
+  CacheAttnParams& p = f.a;
+  p.per_tile = rows / p.group;
+  f.chunks = (a.max_q + p.per_tile - 1) / p.per_tile;
+  p.items = static_cast<int64_t>(a.hk) * a.batch * f.chunks * a.splits;
+  if (p.items > 0x7FFFFFFFll) return -7;
+  f.q = static_cast<const __nv_bfloat16*>(a.q); f.q_ld = a.q_ld;
+  const bool f8 = a.k_scale != nullptr;
+  int r;
+  if (f8) {
+    if (!al16(a.k_scale) || !al16(a.v_scale)) return -5;
+    f.ks = static_cast<const uint8_t*>(a.k_scale); f.vs = static_cast<const uint8_t*>(a.v_scale);
+    r = code_map(&f.tma_k, a, a.k, p.box, a.d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+    if (r == 0) r = code_map(&f.tma_v, a, a.v, p.box, CU_TENSOR_MAP_SWIZZLE_NONE);
+  } else {
+    const int64_t slots = static_cast<int64_t>(a.num_blocks) * a.block;
+    r = page_map(&f.tma_k, a, a.k, slots, p.box);
+    if (r == 0) r = page_map(&f.tma_v, a, a.v, slots, p.box);
+  }
+  if (r != 0) return -20 + r;
   const int sms = sm_count();
   const unsigned grid = static_cast<unsigned>(p.items < sms ? p.items : sms);
-  if (a.d == 128) r = f8 ? run_cache_attn<128, true>(p, grid, stream) : run_cache_attn<128, false>(p, grid, stream);
-  else r = f8 ? run_cache_attn<64, true>(p, grid, stream) : run_cache_attn<64, false>(p, grid, stream);
-  if (r != 0 || a.splits == 1) return r;
-  const unsigned rows = static_cast<unsigned>((a.total_q * a.hq + 3) / 4);
-  (a.d == 128 ? cache_attn_merge_kernel<128> : cache_attn_merge_kernel<64>)<<<rows, 128, 0, stream>>>(p);
-  return static_cast<int>(cudaGetLastError());
+  if (a.d == 128) r = f8 ? run_cache_few<128, true>(f, rows, grid, stream) : run_cache_few<128, false>(f, rows, grid, stream);
+  else r = f8 ? run_cache_few<64, true>(f, rows, grid, stream) : run_cache_few<64, false>(f, rows, grid, stream);
+  return r != 0 || a.splits == 1 ? r : launch_merge(p, a.d, stream);
+}
+
+// One launch over the sequences of `a`; rows of sequences without cu_q begin at first_row.
+int launch_cache_tiles(const CacheAttnArgs& a, int first_row, cudaStream_t stream) {
+  const CacheGrid g = cache_grid(a);
+  CacheAttnParams p = cache_params(a);
+  p.per_tile = g.per_tile;
+  int r = make_tmap_3d(&p.tma_q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.q, static_cast<uint64_t>(a.d), static_cast<uint64_t>(a.hq),
+                       static_cast<uint64_t>(a.total_q), static_cast<uint64_t>(a.d) * 2, static_cast<uint64_t>(a.q_ld) * 2, 64,
+                       static_cast<uint32_t>(p.group), static_cast<uint32_t>(p.per_tile));
+  if (r != 0) return -10 + r;
+  const bool wide = a.k_scale != nullptr;
+  p.room = a.table_width * a.block;
+  const int64_t slots = wide ? static_cast<int64_t>(a.batch) * p.room : static_cast<int64_t>(a.num_blocks) * a.block;
+  if (slots >= (1ll << 31)) return -3;
+  if (wide) {
+    p.box = kCaTile;
+    p.table = nullptr;
+  }
+  r = page_map(&p.tma_k, a, wide ? a.wide_k : a.k, slots, p.box);
+  if (r != 0) return -20 + r;
+  r = page_map(&p.tma_v, a, wide ? a.wide_v : a.v, slots, p.box);
+  if (r != 0) return -30 + r;
+  p.two = g.two; p.items = g.items * a.splits;
+  p.first_row = first_row;
+  if (wide) {
+    CacheWidenArgs w = {a.k, a.v, a.k_scale, a.v_scale, a.wide_k, a.wide_v, a.table, a.lens, a.cu_q, a.table_width, a.block,
+                        a.num_blocks, a.hk, p.room, p.window, p.first, a.status};
+    const int64_t blocks = (static_cast<int64_t>(p.room) * 2 * a.hk * (a.d / 16) + 255) / 256;
+    if (blocks > 0x7FFFFFFFll || a.batch > 65535) return -7;
+    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(a.batch));
+    (a.d == 128 ? cache_widen_kernel<128> : cache_widen_kernel<64>)<<<grid, 256, 0, stream>>>(w);
+    r = static_cast<int>(cudaGetLastError());
+    if (r != 0) return r;
+  }
+  const int sms = sm_count();
+  const unsigned grid = static_cast<unsigned>(p.items < sms ? p.items : sms);
+  r = a.d == 128 ? run_cache_attn<128>(p, grid, stream) : run_cache_attn<64>(p, grid, stream);
+  return r != 0 || a.splits == 1 ? r : launch_merge(p, a.d, stream);
+}
+
+}  // namespace
+
+int launch_cache_attn(const CacheAttnArgs& a, cudaStream_t stream) {
+  if (a.total_q <= 0 || a.batch <= 0) return 0;
+  int r = check(a);
+  if (r != 0) return r;
+  if (a.splits < 1 || (a.splits > 1 && (a.partial_o == nullptr || a.partial_ml == nullptr))) return -6;
+  if (const int few = few_rows(a)) return launch_cache_few(a, few, stream);
+  if (a.k_scale == nullptr) return launch_cache_tiles(a, 0, stream);
+  if (a.wide_k == nullptr || a.wide_v == nullptr || a.wide_batch < 1) return -8;
+  for (int b = 0; b < a.batch && r == 0; b += a.wide_batch) {
+    CacheAttnArgs part = a;
+    part.batch = a.batch - b < a.wide_batch ? a.batch - b : a.wide_batch;
+    part.table += static_cast<int64_t>(b) * a.table_width;
+    part.lens += b;
+    if (a.cu_q != nullptr) part.cu_q += b;
+    part.zero_rest = a.zero_rest && b + part.batch == a.batch;
+    r = launch_cache_tiles(part, b, stream);
+  }
+  return r;
 }
 
 }  // namespace yv

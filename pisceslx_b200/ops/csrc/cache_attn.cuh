@@ -1,5 +1,5 @@
-// Attention of new tokens over cached ones (sm_100a): causal, grouped heads, keys and values in pages of bf16 or of e4m3 codes, an
-// optional window with a few first tokens that stay visible.
+// Attention of new tokens over cached ones (sm_100a): causal, grouped heads, keys and values in bf16 pages (of 8-bit pages what the
+// tokens see is widened to bf16 first, by cache_widen_kernel), an optional window with a few first tokens that stay visible.
 //
 // Query position p of a sequence sees key j <= p if there is no window w, or j > p - w, or j < first.  With n cached tokens, the
 // new ones among them, the last query sits at n - 1.
@@ -13,10 +13,9 @@
 //
 // Roles (the pipeline is that of attention_fwd.cuh):
 //   warps 0..3  softmax of tile 0, warps 4..7 of tile 1 (or of every other key tile): a thread owns a row = a TMEM lane
-//   warp 8      TMA: query tiles; bf16 keys and values, one copy for each `box` rows of a page
+//   warp 8      TMA: query tiles and keys, one copy for each `box` rows of a page; warp 10: values
 //   warp 9      MMA: S = Q K^T (SS), O += P V (TS), one thread's products in order
-//   warps 10,11 give their registers away
-//   warps 12..15 (8-bit pages) fetch codes, make bf16 of them in registers, exactly, and store the tiles as the copies would
+//   warp 11     gives its registers away
 // TMEM columns: [0,128) S0/P0, [128,256) S1/P1, [256,256+D) O0, [384,384+D) O1.
 //
 // What a page holds past the end of a sequence, or in front of everything that the block sees, may be anything: its scores are
@@ -24,23 +23,31 @@
 #pragma once
 #include "attention_math.cuh"
 #include "cache_ops.h"
+#include "chain.cuh"
 #include "per_device.h"
 #include "sm100.cuh"
 #include "tensormap.h"
 
 namespace yv {
 
+struct CacheWidenArgs {
+  const void *k, *v, *k_scale, *v_scale;
+  void *ko, *vo;
+  const int *table, *lens, *cu_q;
+  int table_width, block, num_blocks, hk, room, window, first;
+  uint32_t* status;
+};
+
 struct CacheAttnParams {
   CUtensorMap tma_q;             // (d, query head, token), box (64, G, 128 / G)
-  CUtensorMap tma_k, tma_v;      // bf16: (d, key head, slot), box (64, 1, box)
-  const uint8_t *k8, *v8, *ks, *vs;
+  CUtensorMap tma_k, tma_v;      // (d, key head, slot), box (64, 1, box)
   __nv_bfloat16* o;
   int64_t o_ld;
   float *po, *pml;
-  const int *cu_q, *table, *lens;
+  const int *cu_q, *table, *lens;   // without a table key j of sequence b has the slot b * room + j
   int64_t total_q, items;
   int hq, hk, group, per_tile, batch, max_q, block, box, num_blocks, table_width;
-  int window, first, two, splits, zero_rest;
+  int window, first, two, splits, zero_rest, first_row, room;
   float scale_log2;
   uint32_t* status;
 };
@@ -50,27 +57,75 @@ constexpr int kCaPoly = 4;                      // pairs of 16 whose 2^x is a po
 constexpr float kCaMask = -1.0e30f;
 constexpr float kCaRescale = 8.0f;              // log2 units
 
-template <int D, bool F8>
+template <int D>
 struct CacheAttn {
-  static constexpr int kThreads = F8 ? 512 : 384;
-  // registers of the softmax warps, of warps 8..11 and of warps 12..15: together what the block was launched with
-  static constexpr int kSoftmaxRegs = F8 ? 184 : 208, kOtherRegs = F8 ? 56 : 88, kFetchRegs = 88;
+  static constexpr int kThreads = 384;
+  // registers of the softmax warps and of the others: together what the block was launched with (3 x 168)
+  static constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
   static constexpr int kBytes = kCaTile * D * 2;                     // a tile of Q, K or V
   static constexpr int kStages = D == 64 ? 3 : 2;
   static constexpr int kTotal = kBytes * (2 + 2 * kStages) + kCaTile * 8 + 256 + 1024;
 };
-static_assert(2 * 184 + 56 + 88 == 512 && 2 * 208 + 88 == 3 * 168, "register shares");
 
 // Item of round r of a CTA; every other round runs backwards, so that no CTA gets the heaviest item of each.
 __device__ __forceinline__ int64_t ca_item_of(int64_t r) {
   return r * gridDim.x + ((r & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
 }
 
-struct CacheItem {
+// The key tiles that a block of queries walks, as a list: those of the first tokens, then those from the window's first key on.
+struct CacheTiles {
+  int lo, last, first_end;           // keys that any row of the block sees: [0, first_end) and [lo, last]
+  int ns, w0, begin;                 // tiles in front of the window's first one, that one, first entry of this key range in the list
+
+  // queries at positions from .. to; range `split` of `splits`.  Returns the entry behind the last one.
+  __device__ __forceinline__ int set(int from, int to, int window, int first, int split, int splits) {
+    last = to;
+    lo = window > 0 ? max(from - window + 1, 0) : 0;
+    first_end = window > 0 ? min(first, lo) : 0;
+    w0 = lo / kCaTile;
+    ns = min((first_end + kCaTile - 1) / kCaTile, w0);
+    const int all = list_end(last);
+    begin = static_cast<int>(static_cast<int64_t>(all) * split / splits);
+    return static_cast<int>(static_cast<int64_t>(all) * (split + 1) / splits);
+  }
+  // entries of the list up to the tile with key `k`
+  __device__ __forceinline__ int list_end(int k) const {
+    if (k < 0) return 0;
+    const int tile = k / kCaTile;
+    return tile < w0 ? min(ns, tile + 1) : ns + tile - w0 + 1;
+  }
+  // first key of the tile at a place of the range
+  __device__ __forceinline__ int first_key(int at) const {
+    at += begin;
+    return (at < ns ? at : w0 + at - ns) * kCaTile;
+  }
+  __device__ __forceinline__ bool seen(int key) const { return key <= last && (key >= lo || key < first_end); }
+  // whether any of n keys from `key` on is seen, and whether all of a tile are
+  __device__ __forceinline__ bool any(int key, int n) const { return key <= last && (key + n > lo || key < first_end); }
+  __device__ __forceinline__ bool whole(int key) const {
+    return key + kCaTile - 1 <= last && (key >= lo || key + kCaTile <= first_end);
+  }
+};
+
+// Rows of q and cached tokens of sequence b; what is out of range is reported (by one thread) and counts as empty.
+__device__ __forceinline__ void ca_sequence(const CacheAttnParams& p, int b, int& q_begin, int& q_len, int& k_len) {
+  q_begin = p.cu_q != nullptr ? p.cu_q[b] : p.first_row + b;
+  const int q_end = p.cu_q != nullptr ? p.cu_q[b + 1] : q_begin + 1;
+  q_len = q_end - q_begin;
+  if (q_begin < 0 || q_end > p.total_q || q_len > p.max_q) {
+    if (threadIdx.x == 0 && p.status != nullptr) atomicOr(p.status, kStatusBadArgument);
+    q_len = 0;
+  }
+  k_len = p.lens[b];
+  if (k_len < 0 || static_cast<int64_t>(k_len) > static_cast<int64_t>(p.table_width) * p.block) {
+    if (threadIdx.x == 0 && p.status != nullptr) atomicOr(p.status, kStatusIndexOutOfRange);
+    k_len = 0;
+  }
+}
+
+struct CacheItem : CacheTiles {
   int b, kvh, split;
   int t0, q_begin, q_len, shift;     // first token of the block; a sequence's rows of q; key of query i is i + shift
-  int lo, last, first_end;           // keys that any row of the block sees: [0, first_end) and [lo, last]
-  int ns, w0, begin;                 // tiles in front of the window's first one, that one, first entry of this range in the list
   int n[2];                          // key tiles of the two halves
   bool second, shared;               // there is a second query tile; both halves work on the first
 
@@ -84,32 +139,15 @@ struct CacheItem {
     rest -= b * p.hk * p.splits;
     split = rest / p.hk;
     kvh = rest - split * p.hk;
-    q_begin = p.cu_q != nullptr ? p.cu_q[b] : b;
-    const int q_end = p.cu_q != nullptr ? p.cu_q[b + 1] : b + 1;
-    q_len = q_end - q_begin;
-    if (q_begin < 0 || q_end > p.total_q || q_len > p.max_q) {                   // reported; rows that do not exist are no queries
-      if (threadIdx.x == 0 && p.status != nullptr) atomicOr(p.status, kStatusBadArgument);
-      q_len = 0;
-    }
+    int k_len;
+    ca_sequence(p, b, q_begin, q_len, k_len);
     const int tokens = p.per_tile << p.two;
     const int blk = (q_len + tokens - 1) / tokens - 1 - rank;                    // late (heavy) blocks first
     if (blk < 0) return false;
-    int k_len = p.lens[b];
-    if (k_len < 0 || static_cast<int64_t>(k_len) > static_cast<int64_t>(p.table_width) * p.block) {
-      if (threadIdx.x == 0 && p.status != nullptr) atomicOr(p.status, kStatusIndexOutOfRange);
-      k_len = 0;
-    }
     t0 = blk * tokens;
     second = p.two != 0 && t0 + p.per_tile < q_len;
     shift = k_len - q_len;
-    last = min(t0 + tokens, q_len) - 1 + shift;
-    lo = p.window > 0 ? max(t0 + shift - p.window + 1, 0) : 0;
-    first_end = p.window > 0 ? min(p.first, lo) : 0;
-    w0 = lo / kCaTile;
-    ns = min((first_end + kCaTile - 1) / kCaTile, w0);
-    const int all = list_end(last);
-    begin = static_cast<int>(static_cast<int64_t>(all) * split / p.splits);
-    const int end = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / p.splits);
+    const int end = set(t0 + shift, min(t0 + tokens, q_len) - 1 + shift, p.window, p.first, split, p.splits);
     n[0] = min(max(list_end(min(t0 + p.per_tile, q_len) - 1 + shift) - begin, 0), end - begin);
     n[1] = second ? end - begin : 0;
     shared = !second && n[0] > 1;
@@ -119,31 +157,17 @@ struct CacheItem {
     }
     return true;
   }
-  // entries of the list of tiles up to the one with key `k`
-  __device__ __forceinline__ int list_end(int k) const {
-    if (k < 0) return 0;
-    const int tile = k / kCaTile;
-    return tile < w0 ? min(ns, tile + 1) : ns + tile - w0 + 1;
-  }
   __device__ __forceinline__ int count(int t) const { return t == 0 ? n[0] : n[1]; }
   __device__ __forceinline__ int tiles() const { return shared ? n[0] + n[1] : n[0] > n[1] ? n[0] : n[1]; }
   __device__ __forceinline__ int steps() const { return n[0] > n[1] ? n[0] : n[1]; }
-  // place of a half's step j among the item's tiles; first key of the tile at a place
+  // place of a half's step j among the item's tiles
   __device__ __forceinline__ int place(int t, int j) const { return shared ? 2 * j + t : j; }
-  __device__ __forceinline__ int first_key(int at) const {
-    at += begin;
-    return (at < ns ? at : w0 + at - ns) * kCaTile;
-  }
-  __device__ __forceinline__ bool seen(int key) const { return key <= last && (key >= lo || key < first_end); }
-  // whether every key of the tile is seen by some row
-  __device__ __forceinline__ bool whole(int key) const {
-    return key + kCaTile - 1 <= last && (key >= lo || key + kCaTile <= first_end);
-  }
   __device__ __forceinline__ bool last_reader(int t, int j) const { return shared || t == 1 || j >= n[1]; }
 };
 
 // Flat slot of a key of sequence b; at a table entry outside the pool (reported) some valid one.
 __device__ __forceinline__ int ca_slot(const CacheAttnParams& p, int b, int key) {
+  if (p.table == nullptr) return b * p.room + key;
   const int bi = key / p.block;
   int page = p.table[static_cast<int64_t>(b) * p.table_width + bi];
   if (page < 0 || page >= p.num_blocks) {
@@ -153,45 +177,9 @@ __device__ __forceinline__ int ca_slot(const CacheAttnParams& p, int b, int key)
   return page * p.block + (key - bi * p.block);
 }
 
-// Two e4m3 codes in the high bytes of the halves of t -> the bits of bf16 numbers that are 2^-120 times as large: the exponent and
-// mantissa fields line up (4 + 3 bits above a bf16 mantissa's low 4), subnormal codes become bf16 subnormals.
-__device__ __forceinline__ uint32_t ca_widen(uint32_t t) { return (t & 0x80008000u) | ((t >> 4) & 0x07F007F0u); }
-
-__device__ __forceinline__ uint32_t ca_mul2(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
-}
-
-// Factors that take widened codes to their values 2^E code, E = byte - 127, as bf16 pairs: 2^(120 + E), in two parts where bf16
-// has no such number (E > 7: keys or values beyond 57344).  Byte 255 gives NaN.
-__device__ __forceinline__ uint2 ca_factors(uint32_t byte) {
-  const int f = static_cast<int>(byte) + 120;                        // bf16 exponent field of 2^(120 + E)
-  const uint32_t a = byte == 255u ? 0x7FC0u : static_cast<uint32_t>(min(f, 254)) << 7;
-  const uint32_t b = static_cast<uint32_t>(127 + max(f - 254, 0)) << 7;
-  return make_uint2(a * 0x10001u, byte == 255u ? 0x3F803F80u : b * 0x10001u);
-}
-
-// 16 codes -> 16 bf16 numbers
-__device__ __forceinline__ void ca_values(uint4 c, uint2 f, uint4& lo, uint4& hi) {
-  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-  uint32_t r[8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    r[2 * i] = ca_mul2(ca_widen(__byte_perm(w[i], 0, 0x1404)), f.x);
-    r[2 * i + 1] = ca_mul2(ca_widen(__byte_perm(w[i], 0, 0x3424)), f.x);
-  }
-  if (f.y != 0x3F803F80u) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = ca_mul2(r[i], f.y);
-  }
-  lo = make_uint4(r[0], r[1], r[2], r[3]);
-  hi = make_uint4(r[4], r[5], r[6], r[7]);
-}
-
-template <int D, bool F8>
-__global__ void __launch_bounds__(CacheAttn<D, F8>::kThreads, 1) cache_attn_kernel(const __grid_constant__ CacheAttnParams p) {
-  using S = CacheAttn<D, F8>;
+template <int D>
+__global__ void __launch_bounds__(CacheAttn<D>::kThreads, 1) cache_attn_kernel(const __grid_constant__ CacheAttnParams p) {
+  using S = CacheAttn<D>;
   constexpr int kStages = S::kStages;
   constexpr int kSlabs = D / 64;
   constexpr uint32_t kSlab = kCaTile * 128;            // 128 rows x 64 columns
@@ -199,7 +187,6 @@ __global__ void __launch_bounds__(CacheAttn<D, F8>::kThreads, 1) cache_attn_kern
   constexpr uint32_t kIdescPV = make_idesc_bf16(128, D, false, true);
   constexpr uint32_t kTmemCols = 512;
   constexpr uint32_t kOCol = 256;
-  constexpr uint32_t kFills = F8 ? 4 : 1;              // arrivals that make a tile of keys or values full
 
   extern __shared__ uint8_t ca_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ca_raw) + 1023) & ~uintptr_t(1023));
@@ -227,10 +214,8 @@ __global__ void __launch_bounds__(CacheAttn<D, F8>::kThreads, 1) cache_attn_kern
 
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&p.tma_q);
-    if (!F8) {
-      tma_prefetch_desc(&p.tma_k);
-      tma_prefetch_desc(&p.tma_v);
-    }
+    tma_prefetch_desc(&p.tma_k);
+    tma_prefetch_desc(&p.tma_v);
     for (int t = 0; t < 2; ++t) {
       mbar_init(&q_full[t], 1);
       mbar_init(&q_empty[t], 1);
@@ -239,9 +224,9 @@ __global__ void __launch_bounds__(CacheAttn<D, F8>::kThreads, 1) cache_attn_kern
       mbar_init(&o_full[t], 1);
     }
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(&k_full[s], kFills);
+      mbar_init(&k_full[s], 1);
       mbar_init(&k_empty[s], 1);
-      mbar_init(&v_full[s], kFills);
+      mbar_init(&v_full[s], 1);
       mbar_init(&v_empty[s], 1);
     }
     mbar_init(ml_full, 4);
@@ -253,7 +238,7 @@ __global__ void __launch_bounds__(CacheAttn<D, F8>::kThreads, 1) cache_attn_kern
     tmem_relinquish();
   }
   if (p.zero_rest != 0) {                              // rows that belong to no sequence
-    const int64_t used = p.cu_q != nullptr ? p.cu_q[p.batch] : p.batch;
+    const int64_t used = p.cu_q != nullptr ? p.cu_q[p.batch] : p.first_row + p.batch;
     const int64_t vecs = static_cast<int64_t>(p.hq) * D / 8;
     for (int64_t i = (used < 0 ? 0 : used) * vecs + static_cast<int64_t>(blockIdx.x) * S::kThreads + threadIdx.x; i < p.total_q * vecs;
          i += static_cast<int64_t>(gridDim.x) * S::kThreads)
@@ -264,59 +249,67 @@ __global__ void __launch_bounds__(CacheAttn<D, F8>::kThreads, 1) cache_attn_kern
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
 
-  if (warp >= 8 && warp < 12) regs_give<S::kOtherRegs>();
-  if (warp == 8) {
+  if (warp >= 8) regs_give<S::kOtherRegs>();
+  if (warp == 8 || warp == 10) {
     // ------------------------------------ copies --------------------------------------------
-    if (elect_one()) {
-      bool ok = true;
-      uint32_t kv = 0, nq[2] = {0u, 0u};          // key tiles and Q tiles so far
-      for (int64_t r = 0; r * gridDim.x < p.items && ok; ++r) {
-        CacheItem it;
-        if (!it.load(p, r)) continue;
-        for (int t = 0; t < 2 && ok; ++t) {
-          if (it.count(t) == 0) continue;
-          ok = mbar_wait(&q_empty[t], (nq[t] & 1u) ^ 1u, p.status);
-          if (!ok) break;
-          ++nq[t];
+    // The whole warp walks the items: its lanes look up the slots of the next 32 copies at a time, ahead of their use (looked up one
+    // by one, each costs the latency of a load: 16 streams of 32 pages 168 us).
+    // Keys and values have a warp each: a tile of keys that is wanted early does not wait until the values in front of it have room.
+    const bool keys = warp == 8;
+    const CUtensorMap* map = keys ? &p.tma_k : &p.tma_v;
+    uint64_t *full = keys ? k_full : v_full, *empty = keys ? k_empty : v_empty;
+    uint8_t* ring = keys ? sK : sV;
+    const uint32_t lead = elect_one() ? 1u : 0u;
+    bool ok = true;
+    uint32_t kv = 0, nq[2] = {0u, 0u};            // key tiles and Q tiles so far
+    const int boxes = kCaTile / p.box, per_look = 32 / boxes;              // copies of a tile, tiles of a look
+    for (int64_t r = 0; r * gridDim.x < p.items && ok; ++r) {
+      CacheItem it;
+      if (!it.load(p, r)) continue;
+      const int n = it.tiles();
+      // slot of copy `lane` of the tiles from j0 on; negative where no key of it is seen (the keys stay where they are)
+      auto look = [&](int j0) {
+        const int j = j0 + lane / boxes;
+        if (j >= n) return -1;
+        const int a = it.first_key(j) + (lane % boxes) * p.box;
+        return it.any(a, p.box) ? ca_slot(p, it.b, a) : -1;
+      };
+      int rows = look(0), next = -1;
+      for (int t = 0; t < 2 && ok; ++t) {
+        if (!keys || it.count(t) == 0) continue;
+        ok = mbar_wait_warp(&q_empty[t], (nq[t] & 1u) ^ 1u, p.status);
+        if (!ok) break;
+        ++nq[t];
+        if (lead) {
           mbar_expect_tx(&q_full[t], static_cast<uint32_t>(p.per_tile * p.group) * D * 2);
 #pragma unroll
           for (int c = 0; c < kSlabs; ++c)
             tma_load_3d(sQ + t * S::kBytes + c * kSlab, &p.tma_q, &q_full[t], c * 64, it.kvh * p.group,
                         it.q_begin + it.t0 + (it.shared ? 0 : t * p.per_tile));
         }
-        if (F8) continue;
-        const int n = it.tiles(), boxes = kCaTile / p.box;
-        for (int j = 0; j < n && ok; ++j, ++kv) {
-          const uint32_t s = kv % kStages, ph = (kv / kStages) & 1u;
-          const int key = it.first_key(j);
-          // boxes with a key that is seen: the others stay where they are
-          auto any = [&](int i) {
-            const int a = key + i * p.box;
-            return a <= it.last && (a + p.box > it.lo || a < it.first_end);
-          };
-          uint32_t bytes = 0;
-          for (int i = 0; i < boxes; ++i) bytes += any(i) ? static_cast<uint32_t>(p.box) * D * 2 : 0u;
-          ok = mbar_wait(&k_empty[s], ph ^ 1u, p.status);
-          if (!ok) break;
-          mbar_expect_tx(&k_full[s], bytes);
-          for (int i = 0; i < boxes; ++i) {
-            if (!any(i)) continue;
-            const int row = ca_slot(p, it.b, key + i * p.box);
+        __syncwarp();
+      }
+      for (int j = 0; j < n && ok; ++j, ++kv) {
+        const int in = j % per_look;
+        if (in == 0) {
+          if (j > 0) rows = next;
+          next = look(j + per_look);
+        }
+        const uint32_t s = kv % kStages, ph = (kv / kStages) & 1u;
+        const uint32_t here = __ballot_sync(0xFFFFFFFFu, rows >= 0 && lane / boxes == in);
+        const uint32_t bytes = static_cast<uint32_t>(__popc(here)) * p.box * D * 2;
+        ok = mbar_wait_warp(&empty[s], ph ^ 1u, p.status);
+        if (!ok) break;
+        if (lead) mbar_expect_tx(&full[s], bytes);
+        for (int i = 0; i < boxes; ++i) {
+          const int row = __shfl_sync(0xFFFFFFFFu, rows, in * boxes + i);
+          if (lead && row >= 0) {
 #pragma unroll
             for (int c = 0; c < kSlabs; ++c)
-              tma_load_3d(sK + s * S::kBytes + c * kSlab + i * p.box * 128, &p.tma_k, &k_full[s], c * 64, it.kvh, row);
-          }
-          ok = mbar_wait(&v_empty[s], ph ^ 1u, p.status);
-          if (!ok) break;
-          mbar_expect_tx(&v_full[s], bytes);
-          for (int i = 0; i < boxes; ++i) {
-            if (!any(i)) continue;
-            const int row = ca_slot(p, it.b, key + i * p.box);
-#pragma unroll
-            for (int c = 0; c < kSlabs; ++c)
-              tma_load_3d(sV + s * S::kBytes + c * kSlab + i * p.box * 128, &p.tma_v, &v_full[s], c * 64, it.kvh, row);
+              tma_load_3d(ring + s * S::kBytes + c * kSlab + i * p.box * 128, map, &full[s], c * 64, it.kvh, row);
           }
         }
+        __syncwarp();
       }
     }
   } else if (warp == 9) {
@@ -385,79 +378,6 @@ __global__ void __launch_bounds__(CacheAttn<D, F8>::kThreads, 1) cache_attn_kern
           }
         }
         kv += it.tiles();
-      }
-    }
-  } else if (F8 && warp >= 12) {
-    // ------------------------------------ 8-bit tiles ---------------------------------------
-    regs_give<S::kFetchRegs>();
-    constexpr int kLanes = D / 16;                     // lanes of a row, 16 codes each
-    constexpr int kStep = 128 / kLanes, kRows = kCaTile / kStep;
-    const int c = (threadIdx.x - 384) % kLanes, row0 = (threadIdx.x - 384) / kLanes;
-    // 16 codes fill two 16-byte places of a swizzled row.  Where 8 lanes work on one row, those of the second slab start with the
-    // odd place: the 8 stores then meet 8 different groups of banks.
-    const bool odd_first = D == 128 && c >= 4;
-    bool ok = true;
-    uint32_t kv = 0;
-    for (int64_t r = 0; r * gridDim.x < p.items && ok; ++r) {
-      CacheItem it;
-      if (!it.load(p, r)) continue;
-      const int n = it.tiles();
-      int slot[kRows];                                 // of the tile's rows; negative = not seen
-      uint4 got[kRows];
-      uint32_t byte[kRows];
-      auto find = [&](int j) {
-        const int key = it.first_key(j);
-#pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-          const int k = key + row0 + i * kStep;
-          slot[i] = it.seen(k) ? ca_slot(p, it.b, k) : -1;
-        }
-      };
-      auto fetch = [&](const uint8_t* codes, const uint8_t* scale) {
-#pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-          got[i] = make_uint4(0, 0, 0, 0);
-          byte[i] = 127;
-          if (slot[i] >= 0) {
-            const int page = slot[i] / p.block;
-            got[i] = __ldg(reinterpret_cast<const uint4*>(codes + (static_cast<int64_t>(slot[i]) * p.hk + it.kvh) * D) + c);
-            byte[i] = __ldg(scale + (static_cast<int64_t>(page) * p.hk + it.kvh) * p.block + (slot[i] - page * p.block));
-          }
-        }
-      };
-      auto store = [&](uint8_t* tile) {
-#pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-          const int row = row0 + i * kStep;
-          uint4 a, b;
-          ca_values(got[i], ca_factors(byte[i]), a, b);
-          uint8_t* at = tile + (c / 4) * kSlab + row * 128;
-          const int w = (2 * c) & 7, x = row & 7;
-          *reinterpret_cast<uint4*>(at + (((w + (odd_first ? 1 : 0)) ^ x) << 4)) = odd_first ? b : a;
-          *reinterpret_cast<uint4*>(at + (((w + (odd_first ? 0 : 1)) ^ x) << 4)) = odd_first ? a : b;
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-      };
-      if (n > 0) {
-        find(0);
-        fetch(p.k8, p.ks);
-      }
-      for (int j = 0; j < n && ok; ++j, ++kv) {
-        const uint32_t s = kv % kStages, ph = (kv / kStages) & 1u;
-        ok = mbar_wait_warp(&k_empty[s], ph ^ 1u, p.status);
-        if (!ok) break;
-        store(sK + s * S::kBytes);
-        if (lane == 0) mbar_arrive(&k_full[s]);
-        fetch(p.v8, p.vs);
-        ok = mbar_wait_warp(&v_empty[s], ph ^ 1u, p.status);
-        if (!ok) break;
-        store(sV + s * S::kBytes);
-        if (lane == 0) mbar_arrive(&v_full[s]);
-        if (j + 1 < n) {
-          find(j + 1);
-          fetch(p.k8, p.ks);
-        }
       }
     }
   } else if (warp < 8) {
@@ -558,7 +478,7 @@ __global__ void __launch_bounds__(CacheAttn<D, F8>::kThreads, 1) cache_attn_kern
           const float2 rs = __fadd2_rn(rs2[0], rs2[1]);
           l_sum = l_sum * alpha + (rs.x + rs.y);
         }
-        if (!F8 && !it.whole(key0)) {                 // clear the values of keys that no row sees
+        if (!it.whole(key0)) {                 // clear the values of keys that no row sees
           const uint32_t at = kv + it.place(t, j), s = at % kStages;
           ok = mbar_wait(&v_full[s], (at / kStages) & 1u, p.status);
           ok = __all_sync(0xFFFFFFFFu, ok);
@@ -685,14 +605,84 @@ __global__ void __launch_bounds__(CacheAttn<D, F8>::kThreads, 1) cache_attn_kern
   }
 }
 
+// Two e4m3 codes in the high bytes of the halves of t -> the bits of bf16 numbers that are 2^-120 times as large: the exponent and
+// mantissa fields line up (4 + 3 bits above a bf16 mantissa's low 4), subnormal codes become bf16 subnormals.
+__device__ __forceinline__ uint32_t ca_widen(uint32_t t) { return (t & 0x80008000u) | ((t >> 4) & 0x07F007F0u); }
+
+__device__ __forceinline__ uint32_t ca_mul2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
+// Factors that take widened codes to their values 2^E code, E = byte - 127, as bf16 pairs: 2^(120 + E), in two parts where bf16
+// has no such number (E > 7: keys or values beyond 57344).  Byte 255 gives NaN.
+__device__ __forceinline__ uint2 ca_factors(uint32_t byte) {
+  const int f = static_cast<int>(byte) + 120;                        // bf16 exponent field of 2^(120 + E)
+  const uint32_t a = byte == 255u ? 0x7FC0u : static_cast<uint32_t>(min(f, 254)) << 7;
+  const uint32_t b = static_cast<uint32_t>(127 + max(f - 254, 0)) << 7;
+  return make_uint2(a * 0x10001u, byte == 255u ? 0x3F803F80u : b * 0x10001u);
+}
+
+// 16 codes -> 16 bf16 numbers, exactly
+__device__ __forceinline__ void ca_values(uint4 c, uint2 f, uint4& lo, uint4& hi) {
+  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+  uint32_t r[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    r[2 * i] = ca_mul2(ca_widen(__byte_perm(w[i], 0, 0x1404)), f.x);
+    r[2 * i + 1] = ca_mul2(ca_widen(__byte_perm(w[i], 0, 0x3424)), f.x);
+  }
+  if (f.y != 0x3F803F80u) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = ca_mul2(r[i], f.y);
+  }
+  lo = make_uint4(r[0], r[1], r[2], r[3]);
+  hi = make_uint4(r[4], r[5], r[6], r[7]);
+}
+
+// Keys and values that the new tokens of a sequence see, from 8-bit pages to bf16 rows [sequence, room, hk, D] (what they do not
+// see is left alone).  A group of D / 16 lanes per row.  Bound by bytes: 3 for each number.
+template <int D>
+__global__ void __launch_bounds__(256) cache_widen_kernel(const CacheWidenArgs a) {
+  constexpr int kLanes = D / 16;
+  const int64_t at = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / kLanes;
+  const int lane = threadIdx.x % kLanes, b = blockIdx.y;
+  const int key = static_cast<int>(at / (2 * a.hk));
+  int r = static_cast<int>(at - static_cast<int64_t>(key) * 2 * a.hk);
+  const int n = a.lens[b];
+  if (key >= n || n > a.room) return;                          // a length past the table: reported by the attention kernel
+  const int new_tokens = a.cu_q != nullptr ? a.cu_q[b + 1] - a.cu_q[b] : 1;
+  if (a.window > 0 && key <= n - new_tokens - a.window && key >= a.first) return;
+  const bool val = r >= a.hk;
+  if (val) r -= a.hk;
+  const int bi = key / a.block, off = key - bi * a.block;
+  int page = a.table[static_cast<int64_t>(b) * a.table_width + bi];
+  if (page < 0 || page >= a.num_blocks) {
+    if (lane == 0 && a.status != nullptr) atomicOr(a.status, kStatusIndexOutOfRange);
+    page = 0;
+  }
+  const uint4 c = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(val ? a.v : a.k) +
+                                                       ((static_cast<int64_t>(page) * a.block + off) * a.hk + r) * D) + lane);
+  const uint32_t byte = __ldg(static_cast<const uint8_t*>(val ? a.v_scale : a.k_scale) + (static_cast<int64_t>(page) * a.hk + r) * a.block + off);
+  uint4 lo, hi;
+  ca_values(c, ca_factors(byte), lo, hi);
+  uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(val ? a.vo : a.ko) +
+                                        ((static_cast<int64_t>(b) * a.room + key) * a.hk + r) * D) + 2 * lane;
+  dst[0] = lo;
+  dst[1] = hi;
+}
+
 // Joins the key ranges of a query head: a warp for each of the tokens x hq rows.  A range without a visible key has a sum of zero
 // and is passed over (its part of po was written all the same).
 template <int D>
 __global__ void __launch_bounds__(128) cache_attn_merge_kernel(const CacheAttnParams p) {
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  chain_next();
+  chain_wait();
+  const int begin = p.cu_q != nullptr ? p.cu_q[0] : p.first_row, end = p.cu_q != nullptr ? p.cu_q[p.batch] : p.first_row + p.batch;
+  const int64_t row = static_cast<int64_t>(begin) * p.hq + static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
-  const int64_t rows = (p.cu_q != nullptr ? p.cu_q[p.batch] : p.batch) * static_cast<int64_t>(p.hq);
-  if (row >= rows || row >= p.total_q * p.hq) return;
+  if (begin < 0 || row >= static_cast<int64_t>(end) * p.hq || row >= p.total_q * p.hq) return;
   const int64_t step = p.total_q * p.hq;
   float m = -1.0e29f;
   for (int s = 0; s < p.splits; ++s) m = max_nan(m, p.pml[(s * step + row) * 2]);

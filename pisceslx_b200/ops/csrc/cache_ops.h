@@ -36,10 +36,14 @@ struct CacheAttnArgs {
   int splits = 1;                              // key ranges of a query block, see cache_attn_splits
   bool zero_rest = false;                      // rows of o behind the last sequence are cleared (else left alone)
   float *partial_o = nullptr, *partial_ml = nullptr;   // splits > 1: [splits, total_q, hq, d] and [.., 2]
+  void *wide_k = nullptr, *wide_v = nullptr;   // 8-bit pages: bf16 [wide_batch, table_width * block, hk, d] each
+  int wide_batch = 0;
   uint32_t* status = nullptr;
 };
 // Key ranges that launch_cache_attn wants for these sizes (a rule on shapes, so that a captured call can be replayed).
 int cache_attn_splits(const CacheAttnArgs& a);
+// Sequences at a time whose 8-bit keys and values launch_cache_attn wants room for in bf16 (0: none).
+int cache_attn_wide_batch(const CacheAttnArgs& a);
 int launch_cache_attn(const CacheAttnArgs& a, cudaStream_t stream);
 
 }  // namespace yv
