@@ -152,7 +152,7 @@ int launch_cache_read_fp8(const CacheRowsArgs& a, cudaStream_t stream) {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kFewMost = 128;
+constexpr int kFewMost = 64;
 
 int sm_count() {
   static PerDeviceInt count;
@@ -202,11 +202,13 @@ int run_cache_attn(const CacheAttnParams& p, unsigned grid, cudaStream_t stream)
   return static_cast<int>(cudaGetLastError());
 }
 
-// Rows (token, head of a group) a tile of the kernel for few tokens holds, 0 where cache_attn_kernel takes the call.
+// Rows (token, head of a group) that the kernel for few tokens holds, 0 where cache_attn_kernel takes the call.
 int few_rows(const CacheAttnArgs& a) {
   const int64_t rows = static_cast<int64_t>(a.max_q) * (a.hq / a.hk);
-  if (a.hq / a.hk > 64 || rows > kFewMost) return 0;
-  return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+  if (rows > kFewMost) return 0;
+  int r = 4;
+  while (r < rows) r *= 2;
+  return r;
 }
 
 int page_map(CUtensorMap* m, const CacheAttnArgs& a, const void* pages, int64_t slots, int box) {
@@ -217,15 +219,11 @@ int page_map(CUtensorMap* m, const CacheAttnArgs& a, const void* pages, int64_t 
 
 }  // namespace
 
-int cache_attn_splits(const CacheAttnArgs& a) {
-  if (check(a) != 0 || a.batch <= 0) return 1;
-  CacheGrid g = cache_grid(a);
-  const int sms = sm_count(), few = few_rows(a);
-  if (few != 0) {
-    const int per = few / (a.hq / a.hk);
-    g.two = 1;
-    g.items = static_cast<int64_t>(a.hk) * a.batch * ((a.max_q + per - 1) / per);
-  }
+namespace {
+
+int tile_splits(const CacheAttnArgs& a) {
+  const CacheGrid g = cache_grid(a);
+  const int sms = sm_count();
   int64_t keys = static_cast<int64_t>(a.table_width) * a.block;
   if (a.window > 0) keys = keys < a.window + a.first + a.max_q ? keys : a.window + a.first + a.max_q;
   // steps of an item: key tiles of a block of two query tiles, pairs of key tiles of a lone one
@@ -240,11 +238,28 @@ int cache_attn_splits(const CacheAttnArgs& a) {
   return best;
 }
 
-int cache_attn_wide_batch(const CacheAttnArgs& a) {
-  if (a.k_scale == nullptr || check(a) != 0 || a.batch <= 0 || few_rows(a) != 0) return 0;
-  // about a gigabyte at a time, one sequence at least
-  const int64_t one = static_cast<int64_t>(a.table_width) * a.block * a.hk * a.d * 4, fit = (int64_t(1) << 30) / one;
-  return static_cast<int>(fit < 1 ? 1 : fit < a.batch ? fit : a.batch);
+// Scratch: parts of cut sums, then what is widened or counted.
+int64_t part_bytes(const CacheAttnArgs& a, int few) {
+  const int64_t rows = few != 0 ? static_cast<int64_t>(sm_count()) * 2 * few : a.splits > 1 ? a.total_q * a.hq * a.splits : 0;
+  return (rows * (a.d + 2) * 4 + 255) & ~int64_t(255);
+}
+
+}  // namespace
+
+int64_t cache_attn_plan(CacheAttnArgs& a) {
+  a.wide_batch = 0;
+  if (a.total_q <= 0 || a.batch <= 0 || check(a) != 0) return 0;
+  const int few = few_rows(a);
+  if (few != 0) return part_bytes(a, few) + (kFewSequences + 1) * 4;
+  if (a.splits <= 0) a.splits = tile_splits(a);
+  int64_t bytes = part_bytes(a, 0);
+  if (a.k_scale != nullptr) {
+    // about a gigabyte at a time, one sequence at least
+    const int64_t one = static_cast<int64_t>(a.table_width) * a.block * a.hk * a.d * 4, fit = (int64_t(1) << 30) / one;
+    a.wide_batch = static_cast<int>(fit < 1 ? 1 : fit < a.batch ? fit : a.batch);
+    bytes += one * a.wide_batch;
+  }
+  return bytes;
 }
 
 namespace {
@@ -259,7 +274,6 @@ CacheAttnParams cache_params(const CacheAttnArgs& a) {
   CacheAttnParams p = {};
   p.group = a.hq / a.hk;
   p.o = static_cast<__nv_bfloat16*>(a.o); p.o_ld = a.o_ld;
-  p.po = a.partial_o; p.pml = a.partial_ml;
   p.cu_q = a.cu_q; p.table = a.table; p.lens = a.lens;
   p.total_q = a.total_q;
   p.hq = a.hq; p.hk = a.hk; p.batch = a.batch; p.max_q = a.max_q;
@@ -275,22 +289,27 @@ CacheAttnParams cache_params(const CacheAttnArgs& a) {
   return p;
 }
 
-template <int D, bool F8, int N>
+template <int D, bool F8, int R>
 int run_cache_few(const CacheFewParams& p, unsigned grid, cudaStream_t stream) {
-  using S = CacheFew<D, F8, N>;
+  using S = CacheFew<D, F8, R>;
   static PerDeviceInt configured;
   if (!configured.cur()) {
-    const cudaError_t e = cudaFuncSetAttribute(cache_few_kernel<D, F8, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kTotal);
+    const cudaError_t e = cudaFuncSetAttribute(cache_few_kernel<D, F8, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kTotal);
     if (e != cudaSuccess) return static_cast<int>(e);
     configured.cur() = 1;
   }
-  return launch_chained(cache_few_kernel<D, F8, N>, dim3(grid), dim3(S::kThreads), S::kTotal, stream, 0, p);
+  return launch_chained(cache_few_kernel<D, F8, R>, dim3(grid), dim3(S::kThreads), S::kTotal, stream, 0, p);
 }
 
 template <int D, bool F8>
 int run_cache_few(const CacheFewParams& p, int rows, unsigned grid, cudaStream_t stream) {
-  return rows == 16 ? run_cache_few<D, F8, 16>(p, grid, stream) : rows == 32 ? run_cache_few<D, F8, 32>(p, grid, stream)
-                                                                             : run_cache_few<D, F8, 64>(p, grid, stream);
+  switch (rows) {
+    case 4: return run_cache_few<D, F8, 4>(p, grid, stream);
+    case 8: return run_cache_few<D, F8, 8>(p, grid, stream);
+    case 16: return run_cache_few<D, F8, 16>(p, grid, stream);
+    case 32: return run_cache_few<D, F8, 32>(p, grid, stream);
+    default: return run_cache_few<D, F8, 64>(p, grid, stream);
+  }
 }
 
 int code_map(CUtensorMap* m, const CacheAttnArgs& a, const void* codes, int box, CUtensorMapSwizzle swizzle) {
@@ -299,14 +318,25 @@ int code_map(CUtensorMap* m, const CacheAttnArgs& a, const void* codes, int box,
                       static_cast<uint32_t>(a.d), 1, static_cast<uint32_t>(box), swizzle);
 }
 
-int launch_cache_few(const CacheAttnArgs& a, int rows, cudaStream_t stream) {
+template <int D>
+int launch_join(const CacheFewParams& f, int rows, int ctas, cudaStream_t stream) {
+  auto kernel = rows == 4 ? cache_few_join_kernel<D, 4> : rows == 8 ? cache_few_join_kernel<D, 8> : rows == 16 ? cache_few_join_kernel<D, 16>
+                : rows == 32 ? cache_few_join_kernel<D, 32> : cache_few_join_kernel<D, 64>;
+  return launch_chained(kernel, dim3(f.a.hk, f.a.batch), dim3(128), 0, stream, 0, f, ctas);
+}
+
+// One launch over up to kFewSequences sequences; rows of sequences without cu_q begin at first_row.
+int launch_cache_few(const CacheAttnArgs& a, int rows, int first_row, cudaStream_t stream) {
   CacheFewParams f = {};
   f.a = cache_params(a);
   CacheAttnParams& p = f.a;
-  p.per_tile = rows / p.group;
-  f.chunks = (a.max_q + p.per_tile - 1) / p.per_tile;
-  p.items = static_cast<int64_t>(a.hk) * a.batch * f.chunks * a.splits;
-  if (p.items > 0x7FFFFFFFll) return -7;
+  p.first_row = first_row;
+  const int64_t tiles = (static_cast<int64_t>(a.table_width) * a.block + kCaTile - 1) / kCaTile + 1;
+  if (tiles * a.hk * a.batch > 0x7FFFFFFFll) return -7;
+  const int ctas = sm_count();
+  p.po = static_cast<float*>(a.scratch);
+  p.pml = p.po + static_cast<int64_t>(ctas) * 2 * rows * a.d;
+  f.pre = reinterpret_cast<int*>(p.pml + static_cast<int64_t>(ctas) * 2 * rows * 2);
   f.q = static_cast<const __nv_bfloat16*>(a.q); f.q_ld = a.q_ld;
   const bool f8 = a.k_scale != nullptr;
   int r;
@@ -321,11 +351,13 @@ int launch_cache_few(const CacheAttnArgs& a, int rows, cudaStream_t stream) {
     if (r == 0) r = page_map(&f.tma_v, a, a.v, slots, p.box);
   }
   if (r != 0) return -20 + r;
-  const int sms = sm_count();
-  const unsigned grid = static_cast<unsigned>(p.items < sms ? p.items : sms);
+  // no more CTAs than the table has room for tiles
+  const int64_t most = tiles * a.hk * a.batch / kFewLeast;
+  const unsigned grid = static_cast<unsigned>(most < 1 ? 1 : most < ctas ? most : ctas);
   if (a.d == 128) r = f8 ? run_cache_few<128, true>(f, rows, grid, stream) : run_cache_few<128, false>(f, rows, grid, stream);
   else r = f8 ? run_cache_few<64, true>(f, rows, grid, stream) : run_cache_few<64, false>(f, rows, grid, stream);
-  return r != 0 || a.splits == 1 ? r : launch_merge(p, a.d, stream);
+  if (r != 0) return r;
+  return a.d == 128 ? launch_join<128>(f, rows, grid, stream) : launch_join<64>(f, rows, grid, stream);
 }
 
 // One launch over the sequences of `a`; rows of sequences without cu_q begin at first_row.
@@ -345,14 +377,18 @@ int launch_cache_tiles(const CacheAttnArgs& a, int first_row, cudaStream_t strea
     p.box = kCaTile;
     p.table = nullptr;
   }
-  r = page_map(&p.tma_k, a, wide ? a.wide_k : a.k, slots, p.box);
+  char* wide_k = static_cast<char*>(a.scratch) + part_bytes(a, 0);
+  char* wide_v = wide_k + slots * a.hk * a.d * 2;
+  r = page_map(&p.tma_k, a, wide ? wide_k : a.k, slots, p.box);
   if (r != 0) return -20 + r;
-  r = page_map(&p.tma_v, a, wide ? a.wide_v : a.v, slots, p.box);
+  r = page_map(&p.tma_v, a, wide ? wide_v : a.v, slots, p.box);
   if (r != 0) return -30 + r;
   p.two = g.two; p.items = g.items * a.splits;
   p.first_row = first_row;
+  p.po = static_cast<float*>(a.scratch);
+  p.pml = p.po + (a.splits > 1 ? a.total_q * a.hq * a.splits * a.d : 0);
   if (wide) {
-    CacheWidenArgs w = {a.k, a.v, a.k_scale, a.v_scale, a.wide_k, a.wide_v, a.table, a.lens, a.cu_q, a.table_width, a.block,
+    CacheWidenArgs w = {a.k, a.v, a.k_scale, a.v_scale, wide_k, wide_v, a.table, a.lens, a.cu_q, a.table_width, a.block,
                         a.num_blocks, a.hk, p.room, p.window, p.first, a.status};
     const int64_t blocks = (static_cast<int64_t>(p.room) * 2 * a.hk * (a.d / 16) + 255) / 256;
     if (blocks > 0x7FFFFFFFll || a.batch > 65535) return -7;
@@ -373,18 +409,19 @@ int launch_cache_attn(const CacheAttnArgs& a, cudaStream_t stream) {
   if (a.total_q <= 0 || a.batch <= 0) return 0;
   int r = check(a);
   if (r != 0) return r;
-  if (a.splits < 1 || (a.splits > 1 && (a.partial_o == nullptr || a.partial_ml == nullptr))) return -6;
-  if (const int few = few_rows(a)) return launch_cache_few(a, few, stream);
-  if (a.k_scale == nullptr) return launch_cache_tiles(a, 0, stream);
-  if (a.wide_k == nullptr || a.wide_v == nullptr || a.wide_batch < 1) return -8;
-  for (int b = 0; b < a.batch && r == 0; b += a.wide_batch) {
+  const int few = few_rows(a);
+  if (few == 0 && a.splits < 1) return -6;
+  if (few == 0 && a.k_scale == nullptr) return a.splits > 1 && a.scratch == nullptr ? -8 : launch_cache_tiles(a, 0, stream);
+  const int at_once = few != 0 ? kFewSequences : a.wide_batch;
+  if (a.scratch == nullptr || at_once < 1) return -8;
+  for (int b = 0; b < a.batch && r == 0; b += at_once) {
     CacheAttnArgs part = a;
-    part.batch = a.batch - b < a.wide_batch ? a.batch - b : a.wide_batch;
+    part.batch = a.batch - b < at_once ? a.batch - b : at_once;
     part.table += static_cast<int64_t>(b) * a.table_width;
     part.lens += b;
     if (a.cu_q != nullptr) part.cu_q += b;
     part.zero_rest = a.zero_rest && b + part.batch == a.batch;
-    r = launch_cache_tiles(part, b, stream);
+    r = few != 0 ? launch_cache_few(part, few, b, stream) : launch_cache_tiles(part, b, stream);
   }
   return r;
 }

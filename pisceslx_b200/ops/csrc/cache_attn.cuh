@@ -107,18 +107,18 @@ struct CacheTiles {
   }
 };
 
-// Rows of q and cached tokens of sequence b; what is out of range is reported (by one thread) and counts as empty.
-__device__ __forceinline__ void ca_sequence(const CacheAttnParams& p, int b, int& q_begin, int& q_len, int& k_len) {
+// Rows of q and cached tokens of sequence b; what is out of range is reported (if `report`) and counts as empty.
+__device__ __forceinline__ void ca_sequence(const CacheAttnParams& p, int b, int& q_begin, int& q_len, int& k_len, bool report) {
   q_begin = p.cu_q != nullptr ? p.cu_q[b] : p.first_row + b;
   const int q_end = p.cu_q != nullptr ? p.cu_q[b + 1] : q_begin + 1;
   q_len = q_end - q_begin;
   if (q_begin < 0 || q_end > p.total_q || q_len > p.max_q) {
-    if (threadIdx.x == 0 && p.status != nullptr) atomicOr(p.status, kStatusBadArgument);
+    if (report && p.status != nullptr) atomicOr(p.status, kStatusBadArgument);
     q_len = 0;
   }
   k_len = p.lens[b];
   if (k_len < 0 || static_cast<int64_t>(k_len) > static_cast<int64_t>(p.table_width) * p.block) {
-    if (threadIdx.x == 0 && p.status != nullptr) atomicOr(p.status, kStatusIndexOutOfRange);
+    if (report && p.status != nullptr) atomicOr(p.status, kStatusIndexOutOfRange);
     k_len = 0;
   }
 }
@@ -140,7 +140,7 @@ struct CacheItem : CacheTiles {
     split = rest / p.hk;
     kvh = rest - split * p.hk;
     int k_len;
-    ca_sequence(p, b, q_begin, q_len, k_len);
+    ca_sequence(p, b, q_begin, q_len, k_len, threadIdx.x == 0);
     const int tokens = p.per_tile << p.two;
     const int blk = (q_len + tokens - 1) / tokens - 1 - rank;                    // late (heavy) blocks first
     if (blk < 0) return false;
@@ -615,27 +615,21 @@ __device__ __forceinline__ uint32_t ca_mul2(uint32_t a, uint32_t b) {
   return d;
 }
 
-// Factors that take widened codes to their values 2^E code, E = byte - 127, as bf16 pairs: 2^(120 + E), in two parts where bf16
-// has no such number (E > 7: keys or values beyond 57344).  Byte 255 gives NaN.
-__device__ __forceinline__ uint2 ca_factors(uint32_t byte) {
-  const int f = static_cast<int>(byte) + 120;                        // bf16 exponent field of 2^(120 + E)
-  const uint32_t a = byte == 255u ? 0x7FC0u : static_cast<uint32_t>(min(f, 254)) << 7;
-  const uint32_t b = static_cast<uint32_t>(127 + max(f - 254, 0)) << 7;
-  return make_uint2(a * 0x10001u, byte == 255u ? 0x3F803F80u : b * 0x10001u);
-}
-
-// 16 codes -> 16 bf16 numbers, exactly
-__device__ __forceinline__ void ca_values(uint4 c, uint2 f, uint4& lo, uint4& hi) {
+// 16 codes -> 16 bf16 numbers, exactly: times 2^(120 + E), E = byte - 127.  `most`: no byte of the calling warp's group of rows is
+// above it.  Beyond 134 (E > 7: keys or values past 57344) bf16 has no such factor and it comes in two; 255 gives NaN.
+__device__ __forceinline__ void ca_values(uint4 c, uint32_t most, uint32_t byte, uint4& lo, uint4& hi) {
   const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+  const uint32_t f = (most <= 134u ? (byte + 120u) << 7 : byte == 255u ? 0x7FC0u : min(byte + 120u, 254u) << 7) * 0x10001u;
   uint32_t r[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    r[2 * i] = ca_mul2(ca_widen(__byte_perm(w[i], 0, 0x1404)), f.x);
-    r[2 * i + 1] = ca_mul2(ca_widen(__byte_perm(w[i], 0, 0x3424)), f.x);
+    r[2 * i] = ca_mul2(ca_widen(__byte_perm(w[i], 0, 0x1404)), f);
+    r[2 * i + 1] = ca_mul2(ca_widen(__byte_perm(w[i], 0, 0x3424)), f);
   }
-  if (f.y != 0x3F803F80u) {
+  if (most > 134u) {
+    const uint32_t f2 = (byte == 255u ? 127u : 127u + max(byte, 134u) - 134u) * (0x10001u << 7);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = ca_mul2(r[i], f.y);
+    for (int i = 0; i < 8; ++i) r[i] = ca_mul2(r[i], f2);
   }
   lo = make_uint4(r[0], r[1], r[2], r[3]);
   hi = make_uint4(r[4], r[5], r[6], r[7]);
@@ -666,7 +660,7 @@ __global__ void __launch_bounds__(256) cache_widen_kernel(const CacheWidenArgs a
                                                        ((static_cast<int64_t>(page) * a.block + off) * a.hk + r) * D) + lane);
   const uint32_t byte = __ldg(static_cast<const uint8_t*>(val ? a.v_scale : a.k_scale) + (static_cast<int64_t>(page) * a.hk + r) * a.block + off);
   uint4 lo, hi;
-  ca_values(c, ca_factors(byte), lo, hi);
+  ca_values(c, byte, byte, lo, hi);
   uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(val ? a.vo : a.ko) +
                                         ((static_cast<int64_t>(b) * a.room + key) * a.hk + r) * D) + 2 * lane;
   dst[0] = lo;

@@ -1,24 +1,29 @@
 // Attention of few new tokens over cached ones (sm_100a): decode steps, drafts, short turns.  The arithmetic is that of
-// cache_attn.cuh; the keys are the rows of the products here, so that a tile of 128 of them meets 16, 32 or 64 (token, query head)
-// rows N instead of 128, and what bounds the kernel is the bytes of keys and values:
+// cache_attn.cuh; the keys are the rows of the products here, so that a tile of 128 of them meets R = 4 to 64 (token, query head)
+// rows, N = max(R, 16) columns, instead of 128, and what bounds the kernel is the bytes of keys and values:
 //
 //   S^T[128 keys, N]  = K[128 keys, D] Q[N, D]^T            (SS, K-major)
-//   O^T[D, N]        += V[128 keys, D]^T P[N, 128 keys]^T   (SS, V as stored is MN-major)
+//   O^T[D, N]        += V[128 keys, D]^T P[128 keys, N]     (SS; V as stored and P as a key's thread writes it are MN-major)
 //
 // 8-bit pages: S^T takes the key codes as they are (kind::f8f6f4).  A query row is scaled by a power of two like a cached row and
 // held as two e4m3 numbers, q = q1 + q2 / 16: four bits of the eight that a bf16 number has each, so the two are exact for numbers
 // down to 2^-14 of the row's largest, and within 2^-22 of that one below.  They are 2 N columns of one product; a key's exponent
-// and a row's are factors of the sums.  Values are widened to bf16, exactly, by four warps between the copy and the product (P has
-// to keep weights of very different sizes, for which 4 bits and an exponent of e4m3 are too few).
+// and a row's are factors of the sums.  Value codes are widened to fp16, which holds them all, by four warps between the copy and
+// the product (one conversion for two codes; to bf16, with the exponent in it, took five operations and bounded the kernel); their
+// exponents go into the weights, fp16 too: w = p 2^(E - Eref + 4) with a reference Eref at least E - 3, at most 2^15.  fp16 keeps 11
+// bits of weights down to 2^-18 of the largest, and is off by 2^-29 of it below, where a row of bf16 weights keeps 8 bits.
 //
-// One persistent CTA per SM walks (token chunk, key head, key range, sequence) items; barriers and rings run on across items, so
-// that the copies never stop.  Warps:
-//   0..3   softmax: thread t owns key t of a tile (TMEM lane t of S^T) and output dimension t; the reference maximum of a row is
-//          shared, moves in large steps, and the tile's threads meet at one vote on whether it has to
-//   4, 5   one lane issues S^T (two tiles ahead, two buffers), one the product with the values (two P buffers)
-//   6      TMA: a stage holds a tile of keys and values (and, of 8-bit pages, their exponent bytes)
-//   7      rows of the next item's queries: two buffers
-//   8..11  (8-bit pages) values to bf16, two buffers
+// The key tiles of all sequences and key heads form one line, of which every CTA (one per SM) takes an equal piece: the kernel ends
+// everywhere at the same time whatever the lengths are, and nothing but the lengths on the device decides.  A (sequence, head) that
+// lies in one piece is finished there; one that is cut leaves its unnormalised sums, at most two such parts a CTA, to a
+// second kernel.  Barriers and rings run on across items, so that the copies never stop.  Warps:
+//   0..3, 4..7  softmax of every other tile: thread t owns key t of a tile (TMEM lane t of S^T); the group's reference maximum of a
+//               row is shared and moves in large steps, and the group meets at one vote a tile on whether it has to.  The groups
+//               have sums of their own, joined at the end of an item, where a thread owns output dimension t
+//   8, 9        one lane issues S^T (a buffer for each group), one the product with the values
+//   10          TMA: a stage holds a tile of keys and values (and, of 8-bit pages, their exponent bytes)
+//   11          rows of the next item's queries
+//   12..        (8-bit pages) values to bf16, two buffers
 #pragma once
 #include "cache_attn.cuh"
 #include "chain.cuh"
@@ -30,90 +35,156 @@ struct CacheFewParams {
   const __nv_bfloat16* q;
   int64_t q_ld;
   const uint8_t *ks, *vs;
-  CacheAttnParams a;                 // per_tile = tokens of a chunk, items, splits and what the sequences need
-  int chunks;
+  CacheAttnParams a;                 // po, pml: [CTA][2][R][D] and [CTA][2][R][2]
+  int* pre;                          // [batch + 1] tiles in front of every sequence, for the second kernel
 };
+constexpr int kFewSequences = 512;   // of one launch
+constexpr int kFewLeast = 2;         // tiles of a piece: below, more CTAs cost more than they save
 
-template <int D, bool F8, int N>
+template <int D, bool F8, int R>
 struct CacheFew {
-  static constexpr int kThreads = F8 ? 384 : 256;
+  static constexpr int kN = R < 16 ? 16 : R;
+  static constexpr int kThreads = F8 ? 512 : 384;
+  // registers of the softmax warps and of the others, where 16 rows or more need a split: together what the block was launched with
+  static constexpr int kSoftmaxRegs = F8 ? 168 : 208, kOtherRegs = 88;
   static constexpr int kHalf = kCaTile * D * (F8 ? 1 : 2);           // keys, or values, of a stage
   static constexpr int kStage = 2 * kHalf;                           // values, then keys
-  static constexpr int kQ = 2 * N * D;                               // bf16 rows, or two rows of codes
-  static constexpr int kP = N * kCaTile * 2;
-  static constexpr int kWide = F8 ? kCaTile * D * 2 : 0;             // values in bf16
-  static constexpr int kQBufs = N == 16 ? 2 : 1;                     // what more would take a stage away
+  static constexpr int kQ = 2 * kN * D;                              // bf16 rows, or two rows of codes
+  static constexpr int kP = kN * kCaTile * 2;
+  static constexpr int kWide = F8 ? kCaTile * D * 2 : 0;             // values in fp16
+  static constexpr int kQBufs = kN == 16 ? 2 : 1;                    // what more would take a stage away
   static constexpr int kFixed = kQBufs * kQ + 2 * (kP + kWide);
-  static constexpr int kRest = 256 + 4 * 2 * kCaTile + 10 * N * 4;   // barriers, exponent bytes, row tables
+  static constexpr int kRest = 256 + 4 * 2 * kCaTile + 16 * kN * 4 + 64 + 13 * kFewSequences + 64;   // barriers, exponent bytes, tables
   static constexpr int kMost = (227 * 1024 - 1024 - kRest - kFixed) / kStage;
   static constexpr int kStages = kMost < 4 ? kMost : 4;
   static constexpr int kTotal = kFixed + kStages * kStage + kRest + 1024;
-  static constexpr uint32_t kSCols = F8 ? 2 * N : N;                 // columns of a score buffer
-  static constexpr uint32_t kCols = 2 * kSCols + 2 * N <= 64 ? 64 : 2 * kSCols + 2 * N <= 128 ? 128 : 2 * kSCols + 2 * N <= 256 ? 256 : 512;
-  static_assert(kStages >= 2 && kTotal <= 227 * 1024 && 2 * kSCols + 2 * N <= 512, "room");
+  static constexpr uint32_t kSCols = F8 ? 2 * kN : kN;               // columns of a score buffer
+  static constexpr uint32_t kUsed = 2 * kSCols + 4 * kN;             // and two sums for each group
+  static constexpr uint32_t kCols = kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;
+  static_assert(kStages >= 2 && kTotal <= 227 * 1024 && kUsed <= 512, "room");
+};
+static_assert(2 * 168 + 2 * 88 == 4 * 128 && 2 * 208 + 88 == 3 * 168, "register shares");
+
+// Tiles of the line in front of CTA c of n; `all` < 2^31.
+__device__ __forceinline__ int few_cut(int all, int c, int n) { return static_cast<int>(static_cast<int64_t>(all) * c / n); }
+
+// What the roles know of the sequences, in shared memory.
+struct CacheFewTable {
+  int *pre, *q0, *len;               // [batch + 1] tiles of one head in front of a sequence, first row of q, cached tokens
+  uint8_t* q_len;
 };
 
+// A role's walk along the CTA's piece [at, end) of the line: sequence by sequence, head by head.
 struct CacheFewItem : CacheTiles {
-  int b, kvh, split, t0, q_begin, q_len, shift, n;
-  __device__ __forceinline__ bool load(const CacheFewParams& p, int64_t r) {
-    const int64_t w = ca_item_of(r);
-    if (w >= p.a.items) return false;
-    // chunks of the same keys run at the same time: the second reads them from the L2
-    int rest = static_cast<int>(w);
-    const int chunk = rest % p.chunks;
-    rest /= p.chunks;
-    kvh = rest % p.a.hk;
-    rest /= p.a.hk;
-    split = rest % p.a.splits;
-    b = rest / p.a.splits;
-    int k_len;
-    ca_sequence(p.a, b, q_begin, q_len, k_len);
-    t0 = chunk * p.a.per_tile;
-    if (t0 >= q_len) return false;
-    shift = k_len - q_len;
-    n = set(t0 + shift, min(t0 + p.a.per_tile, q_len) - 1 + shift, p.a.window, p.a.first, split, p.a.splits);
-    n -= begin;
+  int at, start, end;                // place on the line; first and last place of the piece
+  int b, kvh, q_begin, q_len, shift, n;
+  int slot;                          // -1: whole, else which of the CTA's parts
+
+  __device__ __forceinline__ void begin_walk(const CacheAttnParams& p, const CacheFewTable& t, int pieces) {
+    const int all = t.pre[p.batch] * p.hk;
+    start = at = few_cut(all, blockIdx.x, pieces);
+    end = static_cast<int>(blockIdx.x) < pieces ? few_cut(all, blockIdx.x + 1, pieces) : at;
+    int low = 0, high = p.batch;     // the last sequence with pre <= at / hk
+    while (high - low > 1) {
+      const int mid = (low + high) / 2;
+      if (t.pre[mid] * p.hk <= at) low = mid; else high = mid;
+    }
+    b = low;
+  }
+  __device__ __forceinline__ bool next(const CacheAttnParams& p, const CacheFewTable& t) {
+    if (at >= end) return false;
+    while (at >= t.pre[b + 1] * p.hk) ++b;
+    const int tiles = t.pre[b + 1] - t.pre[b], place = at - t.pre[b] * p.hk;
+    kvh = place / tiles;
+    const int from = place - kvh * tiles, count = min(tiles - from, end - at);
+    slot = count == tiles ? -1 : at == start ? 0 : 1;
+    at += count;
+    q_begin = t.q0[b];
+    q_len = t.q_len[b];
+    shift = t.len[b] - q_len;
+    n = set(shift, q_len - 1 + shift, p.window, p.first, 0, 1);
+    begin = from;
+    if (n > 0) n = count;            // a sequence that sees nothing has one place on the line
     return true;
   }
 };
 
-// Swizzled K-major operand whose rows are 64 bytes: groups of 8 rows are 512 bytes apart, 16-byte places are exchanged by bits 1, 2
-// of the row.
-__device__ __forceinline__ uint64_t make_smem_desc_rows64(uint32_t smem_addr) {
+// Descriptor of a swizzled operand: rows of `bytes` 32, 64 or 128, groups of 8 rows one after the other (modes 6, 4, 2).  K-major
+// rows hold consecutive k, MN-major ones consecutive columns of one k.  Within a row the 16-byte places are exchanged by the
+// row's number: few_place.
+template <int BYTES>
+__device__ __forceinline__ uint64_t few_desc(uint32_t smem_addr) {
   uint64_t d = 0;
   d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
   d |= static_cast<uint64_t>(1) << 16;
-  d |= static_cast<uint64_t>(512 >> 4) << 32;
+  d |= static_cast<uint64_t>((8 * BYTES) >> 4) << 32;
   d |= static_cast<uint64_t>(1) << 46;
-  d |= static_cast<uint64_t>(4) << 61;
+  d |= static_cast<uint64_t>(BYTES == 128 ? 2 : BYTES == 64 ? 4 : 6) << 61;
   return d;
 }
+template <int BYTES>
+__device__ __forceinline__ int few_place(int row, int place) {
+  return BYTES == 128 ? place ^ (row & 7) : BYTES == 64 ? place ^ ((row >> 1) & 3) : place ^ ((row >> 2) & 1);
+}
 
-// Barrier over the 128 softmax threads with an OR of `v` (lanes that left a wait at different times are brought together first).
-__device__ __forceinline__ bool few_any(bool v) {
+__device__ __forceinline__ int few_pieces(int tiles, int ctas) { return max(1, min(ctas, tiles / kFewLeast)); }
+
+// 8 e4m3 codes -> 8 fp16 numbers, exactly
+__device__ __forceinline__ uint4 few_halves(uint32_t a, uint32_t b) {
+  uint4 r;
+  asm("{\n"
+      ".reg .b16 l, h;\n"
+      "mov.b32 {l, h}, %4;\n"
+      "cvt.rn.f16x2.e4m3x2 %0, l;\n"
+      "cvt.rn.f16x2.e4m3x2 %1, h;\n"
+      "mov.b32 {l, h}, %5;\n"
+      "cvt.rn.f16x2.e4m3x2 %2, l;\n"
+      "cvt.rn.f16x2.e4m3x2 %3, h;\n"
+      "}\n"
+      : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+      : "r"(a), "r"(b));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t few_pack_half(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// 2^(byte - 127); byte 255 gives NaN
+__device__ __forceinline__ float few_power(uint32_t byte) {
+  return byte == 255u ? __int_as_float(0x7FC00000) : byte == 0u ? __int_as_float(0x00400000) : __int_as_float(static_cast<int>(byte) << 23);
+}
+
+// Barrier over `THREADS` threads with an OR of `v` (lanes that left a wait at different times are brought together first).
+template <int THREADS>
+__device__ __forceinline__ bool few_any(int id, bool v) {
   uint32_t any;
   __syncwarp();
   asm volatile(
       "{\n"
       ".reg .pred pin, pout;\n"
       "setp.ne.u32 pin, %1, 0;\n"
-      "bar.red.or.pred pout, 1, 128, pin;\n"
+      "bar.red.or.pred pout, %2, %3, pin;\n"
       "selp.u32 %0, 1, 0, pout;\n"
       "}\n"
       : "=r"(any)
-      : "r"(static_cast<uint32_t>(v))
+      : "r"(static_cast<uint32_t>(v)), "r"(id), "n"(THREADS)
       : "memory");
   return any != 0u;
 }
 
-template <int D, bool F8, int N>
-__global__ void __launch_bounds__(CacheFew<D, F8, N>::kThreads, 1) cache_few_kernel(const __grid_constant__ CacheFewParams fp) {
-  using S = CacheFew<D, F8, N>;
+template <int D, bool F8, int R>
+__global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_kernel(const __grid_constant__ CacheFewParams fp) {
+  using S = CacheFew<D, F8, R>;
   const CacheAttnParams& p = fp.a;
-  constexpr int kStages = S::kStages;
+  constexpr int kStages = S::kStages, N = S::kN;
   constexpr uint32_t kSlab = kCaTile * 128;                          // 128 rows x 64 columns of bf16
+  constexpr int kPRow = N * 2;                                       // bytes of a key's weights
   constexpr uint32_t kIdescS = F8 ? make_idesc_e4m3(128, 2 * N) : make_idesc_bf16(128, N, false, false);
-  constexpr uint32_t kIdescPV = make_idesc_bf16(128, N, true, false);
+  // the format fields of fp16 are zero
+  constexpr uint32_t kIdescPV = make_idesc_bf16(128, N, true, true) & (F8 ? ~((1u << 7) | (1u << 10)) : ~0u);
+  constexpr bool kShares = R >= 16;
 
   extern __shared__ uint8_t cf_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(cf_raw) + 1023) & ~uintptr_t(1023));
@@ -137,10 +208,16 @@ __global__ void __launch_bounds__(CacheFew<D, F8, N>::kThreads, 1) cache_few_ker
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_empty + 2);
   uint8_t* sByte = reinterpret_cast<uint8_t*>(bars) + 256;                               // [kStages][2][128]
   int* sHi = reinterpret_cast<int*>(sByte + kStages * 2 * kCaTile);                      // [2][N] last visible key of a row, -1 = none
-  float* sFactor = reinterpret_cast<float*>(sHi + 2 * N);                                // [2][N] a row's power of two times the scale
-  float* sM = sFactor + 2 * N;                                                           // [N] reference maxima
-  float* sMax = sM + N;                                                                  // [N] new ones
-  float* sRed = sMax + N;                                                                // [4][N]
+  int* sRow = sHi + 2 * N;                                                               // [2][N] token << 8 | head of the group
+  float* sFactor = reinterpret_cast<float*>(sRow + 2 * N);                               // [2][N] a row's power of two times the scale
+  float* sM = sFactor + 2 * N;                                                           // [2 groups][N] reference maxima
+  float* sRed = sM + 2 * N;                                                              // [2 groups][4][N]; a new maximum goes to [0]
+  int* sTop = reinterpret_cast<int*>(sRed + 8 * N);                                      // [2 groups][8] largest exponent bytes, reference
+  CacheFewTable tab;
+  tab.pre = sTop + 16;
+  tab.q0 = tab.pre + kFewSequences + 1;
+  tab.len = tab.q0 + kFewSequences;
+  tab.q_len = reinterpret_cast<uint8_t*>(tab.len + kFewSequences);
 
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0);
@@ -157,13 +234,13 @@ __global__ void __launch_bounds__(CacheFew<D, F8, N>::kThreads, 1) cache_few_ker
       mbar_init(&pv_done[i], 1);
       mbar_init(&v_full[i], 4);
       mbar_init(&q_full[i], 1);
-      mbar_init(&t_empty[i], 4);
+      mbar_init(&t_empty[i], 8);
       mbar_init(&q_empty[i], 1);
-      mbar_init(&o_empty[i], 4);
+      mbar_init(&o_empty[i], 8);
     }
     fence_barrier_init();
   }
-  if (warp == 0) {
+  if (warp == 8) {
     tmem_alloc(tmem_slot, S::kCols);
     tmem_relinquish();
   }
@@ -171,57 +248,93 @@ __global__ void __launch_bounds__(CacheFew<D, F8, N>::kThreads, 1) cache_few_ker
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
+  // query rows that do not exist stay zero
+  for (int i = tid; i < S::kQBufs * S::kQ / 16; i += S::kThreads) reinterpret_cast<uint4*>(sQ)[i] = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
   // the tensor memory is this kernel's before the next one may begin
   chain_next();
   chain_wait();
   if (p.zero_rest != 0) {                                            // rows that belong to no sequence
-    const int64_t used = p.cu_q != nullptr ? p.cu_q[p.batch] : p.batch, vecs = static_cast<int64_t>(p.hq) * D / 8;
+    const int64_t used = p.cu_q != nullptr ? p.cu_q[p.batch] : p.first_row + p.batch, vecs = static_cast<int64_t>(p.hq) * D / 8;
     for (int64_t i = (used < 0 ? 0 : used) * vecs + static_cast<int64_t>(blockIdx.x) * S::kThreads + tid; i < p.total_q * vecs;
          i += static_cast<int64_t>(gridDim.x) * S::kThreads)
       *reinterpret_cast<uint4*>(p.o + i / vecs * p.o_ld + i % vecs * 8) = make_uint4(0, 0, 0, 0);
   }
+  // Tiles in front of every sequence: each thread adds up a few sequences, the warps scan those sums, and the warps' are added.
+  {
+    const int each = (p.batch + S::kThreads - 1) / S::kThreads, b0 = min(tid * each, p.batch), b1 = min(b0 + each, p.batch);
+    int sum = 0;
+    for (int b = b0; b < b1; ++b) {
+      int q0, q_len, len;
+      ca_sequence(p, b, q0, q_len, len, blockIdx.x == 0);
+      CacheTiles tiles;
+      const int n = tiles.set(len - q_len, len - 1, p.window, p.first, 0, 1);
+      tab.q0[b] = q0;
+      tab.q_len[b] = static_cast<uint8_t>(max(q_len, 0));
+      tab.len[b] = len;
+      tab.pre[b + 1] = q_len > 0 ? max(n, 1) : 0;
+      sum += tab.pre[b + 1];
+    }
+    int scan = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int v = __shfl_up_sync(0xFFFFFFFFu, scan, o);
+      if (lane >= o) scan += v;
+    }
+    int* totals = reinterpret_cast<int*>(sRed);                      // [warps]
+    if (lane == 31) totals[warp] = scan;
+    __syncthreads();
+    int ahead = scan - sum;
+    for (int w = 0; w < warp; ++w) ahead += totals[w];
+    for (int b = b0; b < b1; ++b) {
+      ahead += tab.pre[b + 1];
+      tab.pre[b + 1] = ahead;
+    }
+    if (tid == 0) tab.pre[0] = 0;
+    __syncthreads();
+  }
+  if (blockIdx.x == 0)
+    for (int b = tid; b <= p.batch; b += S::kThreads) fp.pre[b] = tab.pre[b];
+  const int pieces = few_pieces(tab.pre[p.batch] * p.hk, gridDim.x);
 
   auto stage_v = [&](uint32_t s) { return sRing + s * S::kStage; };
   auto stage_k = [&](uint32_t s) { return sRing + s * S::kStage + S::kHalf; };
-  const uint32_t tO = tmem_base + 2 * S::kSCols;                     // two buffers of N columns behind the scores'
+  const uint32_t tO = tmem_base + 2 * S::kSCols;                     // [2 items][2 groups] of N columns behind the scores
 
-  if (warp == 6) {
+  if (kShares && warp >= 8) regs_give<S::kOtherRegs>();
+  if (warp == 10) {
     // ------------------------------------ copies --------------------------------------------
     const uint32_t lead = elect_one() ? 1u : 0u;
     const int boxes = kCaTile / p.box, per_look = 32 / boxes;
     uint32_t g = 0;                                                  // tiles so far
     bool ok = true;
-    for (int64_t r = 0; r * gridDim.x < p.items && ok; ++r) {
-      CacheFewItem it;
-      if (!it.load(fp, r)) continue;
-      // slot of copy `lane` of the tiles from j0 on; negative where no key of it is seen
+    CacheFewItem it;
+    it.begin_walk(p, tab, pieces);
+    while (ok && it.next(p, tab)) {
+      // slot of copy `lane` of the tiles from j0 on, and its place in the page; negative where no key of it is seen
       auto look = [&](int j0) {
-        const int j = j0 + lane / boxes;
-        if (j >= it.n) return -1;
-        const int key = it.first_key(j) + (lane % boxes) * p.box;
-        return it.any(key, p.box) ? ca_slot(p, it.b, key) : -1;
+        const int j = j0 + lane / boxes, key = it.first_key(j) + (lane % boxes) * p.box;
+        return j < it.n && it.any(key, p.box) ? make_int2(ca_slot(p, it.b, key), key % p.block) : make_int2(-1, 0);
       };
-      int rows = look(0), next = -1;
-      for (int j = 0; j < it.n && ok; ++j, ++g) {
-        const int in = j % per_look;
+      int2 rows = look(0), next = make_int2(-1, 0);
+      for (int j = 0, in = 0; j < it.n && ok; ++j, ++g) {
         if (in == 0) {
           if (j > 0) rows = next;
           next = look(j + per_look);
         }
         const uint32_t s = g % kStages;
-        const uint32_t here = __ballot_sync(0xFFFFFFFFu, rows >= 0 && lane / boxes == in);
+        const uint32_t here = __ballot_sync(0xFFFFFFFFu, rows.x >= 0 && lane / boxes == in);
         ok = mbar_wait_warp(&empty[s], ((g / kStages) & 1u) ^ 1u, p.status);
         if (!ok) break;
         if (lead) mbar_expect_tx(&full[s], static_cast<uint32_t>(__popc(here)) * p.box * (F8 ? 2 * D + 2 : 4 * D));
         for (int i = 0; i < boxes; ++i) {
-          const int row = __shfl_sync(0xFFFFFFFFu, rows, in * boxes + i);
+          const int row = __shfl_sync(0xFFFFFFFFu, rows.x, in * boxes + i), off = __shfl_sync(0xFFFFFFFFu, rows.y, in * boxes + i);
           if (!lead || row < 0) continue;
           if constexpr (F8) {
+            const int64_t at = static_cast<int64_t>(row) * p.hk + it.kvh * p.block - off * (p.hk - 1);     // [page][head][place]
             tma_load_3d(stage_k(s) + i * p.box * D, &fp.tma_k, &full[s], 0, it.kvh, row);
-            tma_load_3d(stage_v(s) + i * p.box * D, &fp.tma_v, &full[s], 0, it.kvh, row);
-            const int page = row / p.block;
-            const int64_t at = (static_cast<int64_t>(page) * p.hk + it.kvh) * p.block + (row - page * p.block);
             bulk_load_1d(sByte + s * 2 * kCaTile + i * p.box, fp.ks + at, p.box, &full[s]);
+            tma_load_3d(stage_v(s) + i * p.box * D, &fp.tma_v, &full[s], 0, it.kvh, row);
             bulk_load_1d(sByte + s * 2 * kCaTile + kCaTile + i * p.box, fp.vs + at, p.box, &full[s]);
           } else {
 #pragma unroll
@@ -231,15 +344,16 @@ __global__ void __launch_bounds__(CacheFew<D, F8, N>::kThreads, 1) cache_few_ker
           }
         }
         __syncwarp();
+        in = in + 1 == per_look ? 0 : in + 1;
       }
     }
-  } else if (warp == 7) {
+  } else if (warp == 11) {
     // ------------------------------------ query rows ----------------------------------------
     uint32_t items = 0;
     bool ok = true;
-    for (int64_t r = 0; r * gridDim.x < p.items && ok; ++r) {
-      CacheFewItem it;
-      if (!it.load(fp, r)) continue;
+    CacheFewItem it;
+    it.begin_walk(p, tab, pieces);
+    while (ok && it.next(p, tab)) {
       if (it.n == 0) continue;
       const uint32_t tb = items & 1u, qb = items % S::kQBufs;
       ok = mbar_wait_warp(&q_empty[qb], ((items / S::kQBufs) & 1u) ^ 1u, p.status) &&
@@ -248,24 +362,36 @@ __global__ void __launch_bounds__(CacheFew<D, F8, N>::kThreads, 1) cache_few_ker
       ++items;
       constexpr int E = D / 32;                                      // numbers of a lane
       uint8_t* dst = sQ + qb * S::kQ;
-#pragma unroll 8
-      for (int i = 0; i < N; ++i) {
-        const int tok = i / p.group, h = i - tok * p.group;
-        const bool there = tok < p.per_tile && it.t0 + tok < it.q_len;
-        uint32_t w[E / 2];
+      constexpr int kAhead = R < 16 ? R : 16;                        // rows whose loads are under way together
+#pragma unroll 1
+      for (int i0 = 0; i0 < R; i0 += kAhead) {
+      uint32_t all[kAhead][E / 2];
+      int tok = i0 / p.group, h = i0 - tok * p.group, row_of[kAhead];
 #pragma unroll
-        for (int e = 0; e < E / 2; ++e) w[e] = 0;
+      for (int i = 0; i < kAhead; ++i) {
+        const bool there = tok < it.q_len;
+        row_of[i] = there ? tok << 8 | h : -1;
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e) all[i][e] = 0;
         if (there) {
-          const __nv_bfloat16* src = fp.q + static_cast<int64_t>(it.q_begin + it.t0 + tok) * fp.q_ld +
-                                     static_cast<int64_t>(it.kvh * p.group + h) * D + lane * E;
+          const __nv_bfloat16* src = fp.q + static_cast<int64_t>(it.q_begin + tok) * fp.q_ld + static_cast<int64_t>(it.kvh * p.group + h) * D + lane * E;
           if constexpr (E == 4) {
             const uint2 x = *reinterpret_cast<const uint2*>(src);
-            w[0] = x.x;
-            w[1] = x.y;
+            all[i][0] = x.x;
+            all[i][1] = x.y;
           } else {
-            w[0] = *reinterpret_cast<const uint32_t*>(src);
+            all[i][0] = *reinterpret_cast<const uint32_t*>(src);
           }
         }
+        if (++h == p.group) {
+          h = 0;
+          ++tok;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int i = i0 + k;
+        const uint32_t* w = all[k];
         float factor = p.scale_log2;
         if constexpr (F8) {
           uint32_t top = 0;
@@ -288,39 +414,41 @@ __global__ void __launch_bounds__(CacheFew<D, F8, N>::kThreads, 1) cache_few_ker
             c2 |= static_cast<uint32_t>(b) << (16 * e);
           }
           if (!finite) c1 = c2 = 0;
-          // rows i and N + i
+          // rows i and N + i (N is a multiple of 16: the same exchange of places)
+          const uint32_t at = (few_place<D>(i, (lane * E) >> 4) << 4) + ((lane * E) & 15);
           if constexpr (D == 128) {
-            const uint32_t at = ((((lane >> 2) ^ (i & 7)) << 4) | ((lane & 3) << 2));
-            *reinterpret_cast<uint32_t*>(dst + i * 128 + at) = c1;
-            *reinterpret_cast<uint32_t*>(dst + (N + i) * 128 + at) = c2;
+            *reinterpret_cast<uint32_t*>(dst + i * D + at) = c1;
+            *reinterpret_cast<uint32_t*>(dst + (N + i) * D + at) = c2;
           } else {
-            const uint32_t at = ((((lane >> 3) ^ ((i >> 1) & 3)) << 4) | ((lane & 7) << 1));
-            *reinterpret_cast<uint16_t*>(dst + i * 64 + at) = static_cast<uint16_t>(c1);
-            *reinterpret_cast<uint16_t*>(dst + (N + i) * 64 + at) = static_cast<uint16_t>(c2);
+            *reinterpret_cast<uint16_t*>(dst + i * D + at) = static_cast<uint16_t>(c1);
+            *reinterpret_cast<uint16_t*>(dst + (N + i) * D + at) = static_cast<uint16_t>(c2);
           }
         } else if constexpr (E == 4) {
           const int c = lane >> 1;
-          *reinterpret_cast<uint2*>(dst + (c >> 3) * (N * 128) + i * 128 + (((c & 7) ^ (i & 7)) << 4) + ((lane & 1) << 3)) = make_uint2(w[0], w[1]);
+          *reinterpret_cast<uint2*>(dst + (c >> 3) * (N * 128) + i * 128 + (few_place<128>(i, c & 7) << 4) + ((lane & 1) << 3)) = make_uint2(w[0], w[1]);
         } else {
-          *reinterpret_cast<uint32_t*>(dst + i * 128 + (((lane >> 2) ^ (i & 7)) << 4) + ((lane & 3) << 2)) = w[0];
+          *reinterpret_cast<uint32_t*>(dst + i * 128 + (few_place<128>(i, lane >> 2) << 4) + ((lane & 3) << 2)) = w[0];
         }
         if (lane == 0) {
-          sHi[tb * N + i] = there ? it.t0 + tok + it.shift : -1;
+          sHi[tb * N + i] = row_of[k] >= 0 ? (row_of[k] >> 8) + it.shift : -1;
+          sRow[tb * N + i] = row_of[k];
           sFactor[tb * N + i] = factor;
         }
+      }
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_full[tb]);
     }
-  } else if (warp == 4) {
+  } else if (warp == 8) {
     // ------------------------------------ scores --------------------------------------------
     if (elect_one()) {
       uint32_t g = 0, items = 0;
       bool ok = true;
-      for (int64_t r = 0; r * gridDim.x < p.items && ok; ++r) {
-        CacheFewItem it;
-        if (!it.load(fp, r) || it.n == 0) continue;
+      CacheFewItem it;
+      it.begin_walk(p, tab, pieces);
+      while (ok && it.next(p, tab)) {
+        if (it.n == 0) continue;
         const uint32_t qb = items % S::kQBufs;
         ok = mbar_wait(&q_full[items & 1u], (items >> 1) & 1u, p.status);
         ++items;
@@ -334,17 +462,13 @@ __global__ void __launch_bounds__(CacheFew<D, F8, N>::kThreads, 1) cache_few_ker
           const uint32_t aK = smem_u32(stage_k(s)), tS = tmem_base + sb * S::kSCols;
           if constexpr (F8) {
 #pragma unroll
-            for (int kk = 0; kk < D / 32; ++kk) {
-              if constexpr (D == 128)
-                tc_mma_f8_ss(tS, make_smem_desc(aK + kk * 32, 16, 1024), make_smem_desc(aQ + kk * 32, 16, 1024), kIdescS, kk != 0 ? 1u : 0u);
-              else
-                tc_mma_f8_ss(tS, make_smem_desc_rows64(aK + kk * 32), make_smem_desc_rows64(aQ + kk * 32), kIdescS, kk != 0 ? 1u : 0u);
-            }
+            for (int kk = 0; kk < D / 32; ++kk)
+              tc_mma_f8_ss(tS, few_desc<D>(aK + kk * 32), few_desc<D>(aQ + kk * 32), kIdescS, kk != 0 ? 1u : 0u);
           } else {
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk)
-              tc_mma_f16_ss(tS, make_smem_desc(aK + (kk / 4) * kSlab + (kk % 4) * 32, 16, 1024),
-                            make_smem_desc(aQ + (kk / 4) * (N * 128) + (kk % 4) * 32, 16, 1024), kIdescS, kk != 0 ? 1u : 0u);
+              tc_mma_f16_ss(tS, few_desc<128>(aK + (kk / 4) * kSlab + (kk % 4) * 32), few_desc<128>(aQ + (kk / 4) * (N * 128) + (kk % 4) * 32),
+                            kIdescS, kk != 0 ? 1u : 0u);
           }
           tc_commit(&s_full[sb]);
           if (F8) tc_commit(&empty[s]);
@@ -352,14 +476,15 @@ __global__ void __launch_bounds__(CacheFew<D, F8, N>::kThreads, 1) cache_few_ker
         }
       }
     }
-  } else if (warp == 5) {
+  } else if (warp == 9) {
     // ------------------------------------ weights times values ------------------------------
     if (elect_one()) {
       uint32_t g = 0, items = 0;
       bool ok = true;
-      for (int64_t r = 0; r * gridDim.x < p.items && ok; ++r) {
-        CacheFewItem it;
-        if (!it.load(fp, r) || it.n == 0) continue;
+      CacheFewItem it;
+      it.begin_walk(p, tab, pieces);
+      while (ok && it.next(p, tab)) {
+        if (it.n == 0) continue;
         const uint32_t ob = items & 1u;
         ok = mbar_wait(&o_empty[ob], ((items >> 1) & 1u) ^ 1u, p.status);
         ++items;
@@ -372,265 +497,375 @@ __global__ void __launch_bounds__(CacheFew<D, F8, N>::kThreads, 1) cache_few_ker
           const uint32_t aV = F8 ? smem_u32(sWide + pb * S::kWide) : smem_u32(stage_v(s)), aP = smem_u32(sP + pb * S::kP);
 #pragma unroll
           for (int kk = 0; kk < kCaTile / 16; ++kk)
-            tc_mma_f16_ss(tO + ob * N, make_smem_desc(aV + kk * 2048, kSlab, 1024),
-                          make_smem_desc(aP + (kk / 4) * (N * 128) + (kk % 4) * 32, 16, 1024), kIdescPV, (j | kk) != 0 ? 1u : 0u);
+            tc_mma_f16_ss(tO + (ob * 2 + pb) * N, make_smem_desc(aV + kk * 2048, kSlab, 1024), few_desc<kPRow>(aP + kk * 16 * kPRow), kIdescPV,
+                          j >= 2 || kk != 0 ? 1u : 0u);
           tc_commit(&pv_done[pb]);
           if (!F8) tc_commit(&empty[s]);
         }
       }
     }
-  } else if (F8 && warp >= 8) {
-    // ------------------------------------ values to bf16 ------------------------------------
+  } else if (warp >= 12) {
+    if constexpr (F8) {
+    // ------------------------------------ values to fp16 ------------------------------------
     constexpr int kLanes = D / 16;                                   // lanes of a row, 16 codes each
-    constexpr int kStep = 128 / kLanes;
-    const int c = (tid - 256) % kLanes, row0 = (tid - 256) / kLanes;
+    constexpr int kStep = 128 / kLanes, kRows = kCaTile / kStep;
+    const int c = (tid - 384) % kLanes, row0 = (tid - 384) / kLanes;
     // 16 codes fill two 16-byte places of a swizzled row.  Where 8 lanes work on one row, those of the second slab start with the
-    // odd place: the 8 stores then meet 8 different groups of banks.
-    const bool odd_first = D == 128 && c >= 4;
+    // odd place: the 8 stores then meet 8 different groups of banks.  kStep is a multiple of 8: a thread's rows are all alike.
+    const int w = (2 * c) & 7, odd_first = D == 128 && c >= 4 ? 1 : 0;
+    const uint32_t place0 = (c / 4) * kSlab + row0 * 128 + (((w + odd_first) ^ (row0 & 7)) << 4);
+    const uint32_t place1 = (c / 4) * kSlab + row0 * 128 + (((w + 1 - odd_first) ^ (row0 & 7)) << 4);
     uint32_t g = 0;
     bool ok = true;
-    for (int64_t r = 0; r * gridDim.x < p.items && ok; ++r) {
-      CacheFewItem it;
-      if (!it.load(fp, r)) continue;
+    CacheFewItem it;
+    it.begin_walk(p, tab, pieces);
+    while (ok && it.next(p, tab)) {
       for (int j = 0; j < it.n && ok; ++j, ++g) {
         const uint32_t s = g % kStages, vb = g & 1u;
         const int key0 = it.first_key(j);
-        ok = mbar_wait_warp(&full[s], (g / kStages) & 1u, p.status) &&
-             (g < 2 || mbar_wait_warp(&pv_done[vb], ((g >> 1) & 1u) ^ 1u, p.status));
+        ok = mbar_wait_warp(&full[s], (g / kStages) & 1u, p.status);
         if (!ok) break;
-        const uint8_t* src = stage_v(s);
-        const uint8_t* bytes = sByte + s * 2 * kCaTile + kCaTile;
-        uint8_t* dst = sWide + vb * S::kWide + (c / 4) * kSlab;
-#pragma unroll 4
-        for (int row = row0; row < kCaTile; row += kStep) {
-          uint4 a = make_uint4(0, 0, 0, 0), b = make_uint4(0, 0, 0, 0);
-          if (it.seen(key0 + row))
-            ca_values(*reinterpret_cast<const uint4*>(src + row * D + c * 16), ca_factors(bytes[row]), a, b);
-          uint8_t* at = dst + row * 128;
-          const int w = (2 * c) & 7, x = row & 7;
-          *reinterpret_cast<uint4*>(at + (((w + (odd_first ? 1 : 0)) ^ x) << 4)) = odd_first ? b : a;
-          *reinterpret_cast<uint4*>(at + (((w + (odd_first ? 0 : 1)) ^ x) << 4)) = odd_first ? a : b;
+        const uint8_t* src = stage_v(s) + row0 * D + c * 16;
+        uint4 x[kRows];
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) x[i] = *reinterpret_cast<const uint4*>(src + i * kStep * D);
+        if (!it.whole(key0)) {                                       // values that no row sees are cleared (0 * NaN would be NaN)
+#pragma unroll
+          for (int i = 0; i < kRows; ++i)
+            if (!it.seen(key0 + row0 + i * kStep)) x[i] = make_uint4(0, 0, 0, 0);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[s]);
+        ok = g < 2 || mbar_wait_warp(&pv_done[vb], ((g >> 1) & 1u) ^ 1u, p.status);
+        if (!ok) break;
+        uint8_t* dst = sWide + vb * S::kWide;
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+          const uint4 a = few_halves(x[i].x, x[i].y), b = few_halves(x[i].z, x[i].w);
+          *reinterpret_cast<uint4*>(dst + place0 + i * kStep * 128) = odd_first ? b : a;
+          *reinterpret_cast<uint4*>(dst + place1 + i * kStep * 128) = odd_first ? a : b;
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&v_full[vb]);
-          mbar_arrive(&empty[s]);
-        }
+        if (lane == 0) mbar_arrive(&v_full[vb]);
       }
     }
-  } else if (warp < 4) {
+    }
+  } else if (warp < 8) {
     // ------------------------------------ softmax -------------------------------------------
-    const uint32_t lane_off = static_cast<uint32_t>(warp * 32) << 16;
-    uint32_t g = 0, items = 0;
+    if constexpr (kShares) regs_take<S::kSoftmaxRegs>();
+    const uint32_t grp = warp >> 2;                                  // tiles g with g % 2 == grp
+    const int t = tid & 127, bar = 1 + grp;
+    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem_base + lane_off + grp * S::kSCols;
+    float *m_mine = sM + grp * N, *red = sRed + grp * 4 * N;
+    int* top = sTop + grp * 8;                                       // [0..3] of the warps, [7] the reference byte
+    uint8_t* sp = sP + grp * S::kP + t * kPRow;
+    uint32_t g0 = 0, items = 0;
     bool ok = true;
-    for (int64_t r = 0; r * gridDim.x < p.items; ++r) {
-      CacheFewItem it;
-      if (!it.load(fp, r)) continue;
-      const uint32_t tb = items & 1u;
-      float l[N];
+    CacheFewItem it;
+    it.begin_walk(p, tab, pieces);
+    while (it.next(p, tab)) {
+      const uint32_t tb = items & 1u, ob = items & 1u;
+      const int first = (g0 & 1u) == grp ? 0 : 1;                    // first tile of this group; how many it and the other have
+      const int mine = (it.n - first + 1) / 2;
+      float l[R];
 #pragma unroll
-      for (int i = 0; i < N; ++i) l[i] = 0.f;
+      for (int i = 0; i < R; ++i) l[i] = 0.f;
       if (it.n > 0) {
         ++items;
-        if (tid < N) sM[tid] = -1.0e29f;
+        if (t < R) m_mine[t] = -1.0e29f;
+        if (t == 0) top[7] = -1024;
         ok = mbar_wait(&q_full[tb], ((items - 1) >> 1) & 1u, p.status);
-        ok = !few_any(!ok);                                          // the maxima are set; all agree on whether a wait ran out
-        if (!ok) break;
+        ok = !few_any<128>(bar, !ok);                                // the maxima are set; all agree on whether a wait ran out
       }
       // rows are masked one by one only where some row does not see the whole tile
-      const int hi_least = it.t0 + it.shift, hi_most = min(it.t0 + p.per_tile, it.q_len) - 1 + it.shift;
-      // a warp whose wait ran out walks on, without waiting, to the next vote; all leave there together
-      for (int j = 0; j < it.n; ++j, ++g) {
-        const uint32_t s = g % kStages, sb = g & 1u, ph = (g >> 1) & 1u;
-        const int key0 = it.first_key(j), key = key0 + tid;
-        const bool seen = it.seen(key);
-        const bool all = key0 + kCaTile - 1 <= hi_least &&
+      const int hi_least = it.shift, hi_most = it.q_len - 1 + it.shift;
+      // a warp whose wait ran out walks on, without waiting, to the next vote; the group leaves there together
+      for (int j = first; j < it.n && (ok || j > first); j += 2) {
+        const uint32_t g = g0 + j, s = g % kStages, ph = (g >> 1) & 1u;
+        const int key0 = it.first_key(j), key = key0 + t;
+        const bool seen = it.seen(key), whole = it.whole(key0);
+        const bool all = whole && key0 + kCaTile - 1 <= hi_least &&
                          (p.window == 0 || key0 > hi_most - p.window || key0 + kCaTile <= p.first);
-        ok = ok && mbar_wait(&s_full[sb], ph, p.status);
-        if (F8 || !it.whole(key0)) ok = ok && mbar_wait(&full[s], (g / kStages) & 1u, p.status);
+        ok = ok && mbar_wait(&s_full[grp], ph, p.status);
+        if (F8 || !whole) ok = ok && mbar_wait(&full[s], (g / kStages) & 1u, p.status);
         ok = __all_sync(0xFFFFFFFFu, ok);                            // the aligned tcgen05 instructions need a converged warp
-        float kf = p.scale_log2;
-        if (F8 && ok) {
-          const uint32_t byte = sByte[s * 2 * kCaTile + tid];
-          kf = byte == 255u ? __int_as_float(0x7FC00000) : byte == 0u ? __int_as_float(0x00400000) : __int_as_float(static_cast<int>(byte) << 23);
-        }
-        float sc[N];
+        float sc[R];
         bool high = false;
+        int vbyte = 0;
         if (ok) {
           tc_fence_after_sync();
-          const uint32_t tS = tmem_base + lane_off + sb * S::kSCols;
+          float kf = p.scale_log2;
+          if (F8) {
+            kf = few_power(sByte[s * 2 * kCaTile + t]);
+            vbyte = seen ? sByte[s * 2 * kCaTile + kCaTile + t] : 0;
+            high = vbyte > top[7] + 3 && vbyte != 255;               // NaN needs no reference
+          }
 #pragma unroll
           for (int n0 = 0; n0 < N; n0 += 16) {
+            constexpr int kHere = R < 16 ? R : 16;
             uint32_t a[16];
             tmem_ld16(tS + n0, a);
             if constexpr (F8) {
               uint32_t b[16];
               tmem_ld16(tS + N + n0, b);
-              float f[16];
+              float f[kHere];
 #pragma unroll
-              for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4*>(f + i) = *reinterpret_cast<const float4*>(sFactor + tb * N + n0 + i);
+              for (int i = 0; i < kHere; i += 4) *reinterpret_cast<float4*>(f + i) = *reinterpret_cast<const float4*>(sFactor + tb * N + n0 + i);
               tc_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 16; ++i)
+              for (int i = 0; i < kHere; ++i)
                 sc[n0 + i] = fmaf(__uint_as_float(b[i]), 0.0625f, __uint_as_float(a[i])) * (kf * f[i]);
             } else {
               tc_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) sc[n0 + i] = __uint_as_float(a[i]) * kf;
+              for (int i = 0; i < kHere; ++i) sc[n0 + i] = __uint_as_float(a[i]) * kf;
             }
           }
-          if (!all || !seen) {
+          if (!all) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
+            for (int i = 0; i < R; ++i) {
               const int hi = sHi[tb * N + i];
-              const bool mine = seen && key <= hi && (p.window == 0 || key > hi - p.window || key < p.first);
-              if (!mine) sc[i] = kCaMask;
+              if (!(seen && key <= hi && (p.window == 0 || key > hi - p.window || key < p.first))) sc[i] = kCaMask;
             }
           }
 #pragma unroll
-          for (int i = 0; i < N; i += 4) {
-            const float4 m = *reinterpret_cast<const float4*>(sM + i);
+          for (int i = 0; i < R; i += 4) {
+            const float4 m = *reinterpret_cast<const float4*>(m_mine + i);
             high |= !(sc[i] <= m.x + kCaRescale) || !(sc[i + 1] <= m.y + kCaRescale) || !(sc[i + 2] <= m.z + kCaRescale) ||
                     !(sc[i + 3] <= m.w + kCaRescale);
           }
         }
         tc_fence_before_sync();
         // lazy: a reference maximum moves only when a score exceeds it by more than 2^8 (or is NaN)
-        if (few_any(high || !ok)) {
+        const bool moves = few_any<128>(bar, high || !ok);
+        // the product of the group's last tile has landed: its P buffer is free, its sums may be rescaled
+        if (g >= 2) ok = ok && mbar_wait(&pv_done[grp], ph ^ 1u, p.status);
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (moves) {
           if (ok) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
+            for (int i = 0; i < R; ++i) {
               float v = sc[i];
 #pragma unroll
               for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
-              if (lane == 0) sRed[warp * N + i] = v;
+              if (lane == 0) red[(warp & 3) * N + i] = v;
+            }
+            if (F8) {
+              const int v = __reduce_max_sync(0xFFFFFFFFu, vbyte == 255 ? 0 : vbyte);
+              if (lane == 0) top[warp & 3] = v;
             }
           }
-          ok = !few_any(!ok);
+          ok = !few_any<128>(bar, !ok);
           if (!ok) break;
-          if (tid < N) {
-            const float top = max_nan(max_nan(sRed[tid], sRed[N + tid]), max_nan(sRed[2 * N + tid], sRed[3 * N + tid]));
-            sMax[tid] = !(top <= sM[tid] + kCaRescale) ? top : sM[tid];
+          // a reference exponent that is passed by more than 3 moves as the maxima do
+          const int old_ref = F8 ? top[7] : 0, most = F8 ? max(max(top[0], top[1]), max(top[2], top[3])) : 0;
+          const int ref = most > old_ref + 3 ? most : old_ref;
+          const float rescale = F8 ? ex2(static_cast<float>(old_ref - ref)) : 1.f;
+          if (t < R) {
+            const float top = max_nan(max_nan(red[t], red[N + t]), max_nan(red[2 * N + t], red[3 * N + t]));
+            red[t] = !(top <= m_mine[t] + kCaRescale) ? top : m_mine[t];
           }
-          // the products so far have landed
-          if (j > 0) ok = mbar_wait(&pv_done[(g - 1) & 1u], ((g - 1) >> 1) & 1u, p.status);
-          ok = !few_any(!ok);
-          if (!ok) break;
+          few_any<128>(bar, false);
           tc_fence_after_sync();
+          const uint32_t to = tO + lane_off + (ob * 2 + grp) * N;
 #pragma unroll
           for (int n0 = 0; n0 < N; n0 += 16) {
+            constexpr int kHere = R < 16 ? R : 16;
             uint32_t o[16];
-            if (j > 0) {
-              tmem_ld16(tO + lane_off + ((items - 1) & 1u) * N + n0, o);
+            if (j > first) {
+              tmem_ld16(to + n0, o);
               tc_wait_ld();
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float alpha = ex2(sM[n0 + i] - sMax[n0 + i]);
+            for (int i = 0; i < kHere; ++i) {
+              const float alpha = ex2(m_mine[n0 + i] - red[n0 + i]);
               l[n0 + i] *= alpha;
-              if (j > 0) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              if (j > first) o[i] = __float_as_uint(__uint_as_float(o[i]) * (F8 ? alpha * rescale : alpha));
             }
-            if (j > 0) {
-              tmem_st16(tO + lane_off + ((items - 1) & 1u) * N + n0, o);
+            if (j > first) {
+              tmem_st16(to + n0, o);
               tc_wait_st();
             }
           }
           tc_fence_before_sync();
-          few_any(false);                                            // everyone has read the old maxima
-          if (tid < N) sM[tid] = sMax[tid];
-          few_any(false);
-        }
-        if (g >= 2) {                                                // this P buffer was read by the product of tile g - 2
-          ok = ok && mbar_wait(&pv_done[sb], ph ^ 1u, p.status);
-          ok = __all_sync(0xFFFFFFFFu, ok);
+          few_any<128>(bar, false);                                  // everyone has read the old maxima
+          if (t < R) m_mine[t] = red[t];
+          if (F8 && t == 0) top[7] = ref;
+          few_any<128>(bar, false);
         }
         if (ok) {
-          uint8_t* sp = sP + sb * S::kP + (tid >> 6) * (N * 128) + ((tid & 7) << 1);
+          // A key's weights are a row of P.  The sums take bf16 weights as rounded, as the tensor core multiplies them; fp16 ones, which
+          // hold the value's exponent as well, before they are rounded.
+          uint32_t w[R / 2];
+          const float vf = vbyte == 255 ? __int_as_float(0x7FC00000) : ex2(static_cast<float>(vbyte - top[7] + 4));
 #pragma unroll
-          for (int i0 = 0; i0 < N; i0 += 4) {
-            float m[4];
-            *reinterpret_cast<float4*>(m) = *reinterpret_cast<const float4*>(sM + i0);
+          for (int i = 0; i < R; i += 4) {
+            const float4 m = *reinterpret_cast<const float4*>(m_mine + i);
+            const float e[4] = {ex2(sc[i] - m.x), ex2(sc[i + 1] - m.y), ex2(sc[i + 2] - m.z), ex2(sc[i + 3] - m.w)};     // masked: 0
 #pragma unroll
-            for (int i = i0; i < i0 + 4; ++i) {
-              const __nv_bfloat16 w = __float2bfloat16(ex2(sc[i] - m[i - i0]));          // masked: 2^(-1e30 - m) = 0
-              *reinterpret_cast<__nv_bfloat16*>(sp + i * 128 + ((((tid & 63) >> 3) ^ (i & 7)) << 4)) = w;
-              l[i] += __bfloat162float(w);           // the sum takes the rounded weights that the tensor core multiplies
+            for (int h = 0; h < 2; ++h) {
+              if constexpr (F8) {
+                w[i / 2 + h] = few_pack_half(e[2 * h] * vf, e[2 * h + 1] * vf);
+                l[i + 2 * h] += e[2 * h];
+                l[i + 2 * h + 1] += e[2 * h + 1];
+              } else {
+                w[i / 2 + h] = pack_bf16(e[2 * h], e[2 * h + 1]);
+                l[i + 2 * h] += __uint_as_float(w[i / 2 + h] << 16);
+                l[i + 2 * h + 1] += __uint_as_float(w[i / 2 + h] & 0xFFFF0000u);
+              }
             }
           }
-          if (!F8 && !it.whole(key0)) {
-            if (!seen) {                             // values that no row sees are cleared (0 * NaN would be NaN)
+          if constexpr (R == 4) {
+            *reinterpret_cast<uint2*>(sp + (few_place<kPRow>(t, 0) << 4)) = make_uint2(w[0], w[1]);
+          } else {
 #pragma unroll
-              for (int c = 0; c < D / 64; ++c)
+            for (int i = 0; i < R / 8; ++i)
+              *reinterpret_cast<uint4*>(sp + (few_place<kPRow>(t, i) << 4)) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+          }
+          if (!F8 && !whole && !seen) {              // values that no row sees are cleared (0 * NaN would be NaN)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) reinterpret_cast<uint4*>(stage_v(s) + c * kSlab + tid * 128)[i] = make_uint4(0, 0, 0, 0);
-            }
+            for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+              for (int i = 0; i < 8; ++i) reinterpret_cast<uint4*>(stage_v(s) + c * kSlab + t * 128)[i] = make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async_smem();
           tc_fence_before_sync();
           __syncwarp();
           if (lane == 0) {
-            mbar_arrive(&p_full[sb]);
+            mbar_arrive(&p_full[grp]);
             if (F8) mbar_arrive(&empty[s]);
           }
         }
       }
       if (it.n > 0) {
-        if (ok) ok = mbar_wait(&pv_done[(g - 1) & 1u], ((g - 1) >> 1) & 1u, p.status);
+        const uint32_t end = g0 + first + 2 * mine - 2;              // this group's last tile
+        if (mine > 0) ok = ok && mbar_wait(&pv_done[grp], (end >> 1) & 1u, p.status);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
+        for (int i = 0; i < R; ++i) {
           float v = l[i];
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-          if (lane == 0) sRed[warp * N + i] = v;
+          if (lane == 0) red[(warp & 3) * N + i] = v;
         }
-        ok = !few_any(!ok);
+        ok = !few_any<256>(3, !ok);
         if (!ok) break;                              // a wait ran out (the status word says so): the outputs are not written
         tc_fence_after_sync();
       }
-      const int64_t step = p.total_q * p.hq;
+      // The groups' sums are joined, half of the rows by each group.  A group without a tile has the sum zero, and no product.
+      const bool has0 = it.n > 0 && (it.n > 1 || (g0 & 1u) == 0u), has1 = it.n > 0 && (it.n > 1 || (g0 & 1u) == 1u);
+      const float ref0 = F8 ? few_power(max(sTop[7], 0)) * 0.0625f : 1.f, ref1 = F8 ? few_power(max(sTop[15], 0)) * 0.0625f : 1.f;
+      constexpr int kHalfRows = R / 2, kAtOnce = kHalfRows < 16 ? kHalfRows : 16;
 #pragma unroll 1
-      for (int n0 = 0; n0 < N; n0 += 16) {
-        uint32_t o[16];
-        if (it.n > 0) {
-          tmem_ld16(tO + lane_off + ((items - 1) & 1u) * N + n0, o);
-          tc_wait_ld();
-        } else {
+      for (int part = 0; part < kHalfRows; part += kAtOnce) {
+        const int r0 = static_cast<int>(grp) * kHalfRows + part;     // first row
+        const int n0 = r0 & ~15;
+        uint32_t o0[16], o1[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] = 0u;
+        for (int i = 0; i < 16; ++i) o0[i] = o1[i] = 0u;
+        if (it.n > 0) {
+          if (has0) tmem_ld16(tO + lane_off + (ob * 2) * N + n0, o0);
+          if (has1) tmem_ld16(tO + lane_off + (ob * 2 + 1) * N + n0, o1);
+          tc_wait_ld();
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const int row = n0 + i, tok = row / p.group, h = row - tok * p.group;
-          if (tok >= p.per_tile || it.t0 + tok >= it.q_len) continue;
-          const int64_t at = it.q_begin + it.t0 + tok;
-          const int head = it.kvh * p.group + h;
-          const float sum = it.n > 0 ? sRed[row] + sRed[N + row] + sRed[2 * N + row] + sRed[3 * N + row] : 0.f;
-          if (p.splits > 1) {
-            const int64_t part = it.split * step + at * p.hq + head;
-            if (tid < D) p.po[part * D + tid] = __uint_as_float(o[i]);
-            if (tid == 0) *reinterpret_cast<float2*>(p.pml + part * 2) = make_float2(it.n > 0 ? sM[row] : -1.0e29f, sum);
-          } else if (tid < D) {
-            p.o[at * p.o_ld + static_cast<int64_t>(head) * D + tid] = __float2bfloat16(sum > 0.f ? __uint_as_float(o[i]) / sum : __uint_as_float(o[i]) * 0.f);
+          if (kAtOnce < 16 && (i >= R || (i >= kHalfRows) != (grp != 0))) continue;
+          const int row = n0 + i;
+          int tok, h;
+          float sum = 0.f, f0 = 0.f, f1 = 0.f, m = -1.0e29f;
+          if (it.n > 0) {
+            const int at = sRow[tb * N + row];
+            if (at < 0) continue;
+            tok = at >> 8;
+            h = at & 255;
+            m = max_nan(sM[row], sM[N + row]);
+            f0 = ex2(sM[row] - m);
+            f1 = ex2(sM[N + row] - m);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) sum += sRed[q * N + row] * f0 + sRed[(4 + q) * N + row] * f1;
+            if (F8) {                                                // 2^(Eref - 4)
+              f0 *= has0 ? ref0 : 0.f;
+              f1 *= has1 ? ref1 : 0.f;
+            }
+          } else {
+            tok = row / p.group;
+            h = row - tok * p.group;
+            if (tok >= it.q_len) continue;
+          }
+          const float o = __uint_as_float(o0[i]) * f0 + __uint_as_float(o1[i]) * f1;
+          if (it.slot >= 0) {
+            const int64_t part = (static_cast<int64_t>(blockIdx.x) * 2 + it.slot) * R + row;
+            if (t < D) p.po[part * D + t] = o;
+            if (t == 0) *reinterpret_cast<float2*>(p.pml + part * 2) = make_float2(m, sum);
+          } else if (t < D) {
+            p.o[(it.q_begin + tok) * p.o_ld + static_cast<int64_t>(it.kvh * p.group + h) * D + t] =
+                __float2bfloat16(sum > 0.f ? o / sum : o * 0.f);
           }
         }
       }
       if (it.n > 0) {
         tc_fence_before_sync();
-        few_any(false);                              // sRed, sM and the row tables have been read
+        few_any<256>(3, false);                      // sRed, sM and the row tables have been read
         if (lane == 0) {
-          mbar_arrive(&o_empty[(items - 1) & 1u]);
+          mbar_arrive(&o_empty[ob]);
           mbar_arrive(&t_empty[tb]);
         }
       }
+      g0 += it.n;
     }
   }
 
   tc_fence_before_sync();
   block_settle(p.status);                            // begins with a barrier
-  if (warp == 0) {
+  if (warp == 8) {
     tc_fence_after_sync();
     tmem_dealloc(tmem_base, S::kCols);
+  }
+}
+
+// Joins the parts of a (sequence, head) that was cut: a block for each, most of which leave at once.
+template <int D, int R>
+__global__ void __launch_bounds__(128) cache_few_join_kernel(const CacheFewParams fp, int ctas) {
+  const CacheAttnParams& p = fp.a;
+  chain_next();
+  chain_wait();
+  const int b = blockIdx.y, kvh = blockIdx.x;
+  const int all = fp.pre[p.batch] * p.hk, pieces = few_pieces(all, ctas);
+  const int tiles = fp.pre[b + 1] - fp.pre[b], from = fp.pre[b] * p.hk + kvh * tiles;
+  if (tiles == 0) return;
+  // the piece of a place x is the last one whose cut is not behind it
+  auto piece = [&](int x) {
+    int c = static_cast<int>((static_cast<int64_t>(x) * pieces + pieces - 1) / all);
+    while (c > 0 && few_cut(all, c, pieces) > x) --c;
+    while (few_cut(all, c + 1, pieces) <= x) ++c;
+    return c;
+  };
+  const int c0 = piece(from), c1 = piece(from + tiles - 1);
+  if (c0 == c1) return;
+  const int first_slot = few_cut(all, c0, pieces) == from ? 0 : 1;
+  int q_begin, q_len, k_len;
+  ca_sequence(p, b, q_begin, q_len, k_len, false);
+  constexpr int kGroups = 128 / (D / 4);                             // rows at a time, four numbers a thread
+  const int d4 = threadIdx.x % (D / 4);
+  for (int row = threadIdx.x / (D / 4); row < q_len * p.group; row += kGroups) {
+    float m = -1.0e29f, l = 0.f;
+    for (int c = c0; c <= c1; ++c) m = max_nan(m, p.pml[((c * 2 + (c == c0 ? first_slot : 0)) * R + row) * 2]);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int c = c0; c <= c1; ++c) {
+      const int64_t part = (c * 2 + (c == c0 ? first_slot : 0)) * R + row;
+      const float2 ml = *reinterpret_cast<const float2*>(p.pml + part * 2);
+      const float f = ex2(ml.x - m);
+      const float4 o = *reinterpret_cast<const float4*>(p.po + part * D + d4 * 4);
+      l += ml.y * f;
+      acc.x += o.x * f; acc.y += o.y * f; acc.z += o.z * f; acc.w += o.w * f;
+    }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const int tok = row / p.group, h = row - tok * p.group;
+    *reinterpret_cast<uint2*>(p.o + (q_begin + tok) * p.o_ld + static_cast<int64_t>(kvh * p.group + h) * D + d4 * 4) =
+        make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
   }
 }
 

@@ -33,17 +33,15 @@ struct CacheAttnArgs {
   int batch = 0, max_q = 0, hq = 0, hk = 0, d = 0, block = 0, num_blocks = 0, table_width = 0;
   int window = 0, first = 0;                   // 0 = no window
   float scale = 1.f;
-  int splits = 1;                              // key ranges of a query block, see cache_attn_splits
+  int splits = 1;                              // key ranges of a query block, see cache_attn_plan
   bool zero_rest = false;                      // rows of o behind the last sequence are cleared (else left alone)
-  float *partial_o = nullptr, *partial_ml = nullptr;   // splits > 1: [splits, total_q, hq, d] and [.., 2]
-  void *wide_k = nullptr, *wide_v = nullptr;   // 8-bit pages: bf16 [wide_batch, table_width * block, hk, d] each
+  void* scratch = nullptr;                     // as many bytes as the plan says
   int wide_batch = 0;
   uint32_t* status = nullptr;
 };
-// Key ranges that launch_cache_attn wants for these sizes (a rule on shapes, so that a captured call can be replayed).
-int cache_attn_splits(const CacheAttnArgs& a);
-// Sequences at a time whose 8-bit keys and values launch_cache_attn wants room for in bf16 (0: none).
-int cache_attn_wide_batch(const CacheAttnArgs& a);
+// Decides, from sizes alone (so that a captured call can be replayed), how a call runs: splits (where they are 0) and wide_batch are
+// set; returns the bytes of scratch that it takes.
+int64_t cache_attn_plan(CacheAttnArgs& a);
 int launch_cache_attn(const CacheAttnArgs& a, cudaStream_t stream);
 
 }  // namespace yv
