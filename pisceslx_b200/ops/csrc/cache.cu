@@ -211,10 +211,17 @@ int few_rows(const CacheAttnArgs& a) {
   return r;
 }
 
+// What a miss fetches into the L2: no more than a row of one head.  Another head's is read by another SM, at another time (8-bit
+// rows of 128 bytes, 64 sequences of 3000 tokens: 604 MB read where 414 are needed).
+CUtensorMapL2promotion row_fetch(int bytes) {
+  return bytes >= 256 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : bytes >= 128 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_64B;
+}
+
 int page_map(CUtensorMap* m, const CacheAttnArgs& a, const void* pages, int64_t slots, int box) {
   return make_tmap_3d(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, pages, static_cast<uint64_t>(a.d), static_cast<uint64_t>(a.hk),
                       static_cast<uint64_t>(slots), static_cast<uint64_t>(a.d) * 2,
-                      static_cast<uint64_t>(a.hk) * a.d * 2, 64, 1, static_cast<uint32_t>(box));
+                      static_cast<uint64_t>(a.hk) * a.d * 2, 64, 1, static_cast<uint32_t>(box), CU_TENSOR_MAP_SWIZZLE_128B,
+                      row_fetch(a.d * 2));
 }
 
 }  // namespace
@@ -240,7 +247,7 @@ int tile_splits(const CacheAttnArgs& a) {
 
 // Scratch: parts of cut sums, then what is widened or counted.
 int64_t part_bytes(const CacheAttnArgs& a, int few) {
-  const int64_t rows = few != 0 ? static_cast<int64_t>(sm_count()) * 2 * few : a.splits > 1 ? a.total_q * a.hq * a.splits : 0;
+  const int64_t rows = few != 0 ? static_cast<int64_t>(sm_count()) * 4 * few : a.splits > 1 ? a.total_q * a.hq * a.splits : 0;
   return (rows * (a.d + 2) * 4 + 255) & ~int64_t(255);
 }
 
@@ -315,7 +322,7 @@ int run_cache_few(const CacheFewParams& p, int rows, unsigned grid, cudaStream_t
 int code_map(CUtensorMap* m, const CacheAttnArgs& a, const void* codes, int box, CUtensorMapSwizzle swizzle) {
   return make_tmap_3d(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes, static_cast<uint64_t>(a.d), static_cast<uint64_t>(a.hk),
                       static_cast<uint64_t>(a.num_blocks) * a.block, static_cast<uint64_t>(a.d), static_cast<uint64_t>(a.hk) * a.d,
-                      static_cast<uint32_t>(a.d), 1, static_cast<uint32_t>(box), swizzle);
+                      static_cast<uint32_t>(a.d), 1, static_cast<uint32_t>(box), swizzle, row_fetch(a.d));
 }
 
 template <int D>
@@ -335,8 +342,8 @@ int launch_cache_few(const CacheAttnArgs& a, int rows, int first_row, cudaStream
   if (tiles * a.hk * a.batch > 0x7FFFFFFFll) return -7;
   const int ctas = sm_count();
   p.po = static_cast<float*>(a.scratch);
-  p.pml = p.po + static_cast<int64_t>(ctas) * 2 * rows * a.d;
-  f.pre = reinterpret_cast<int*>(p.pml + static_cast<int64_t>(ctas) * 2 * rows * 2);
+  p.pml = p.po + static_cast<int64_t>(ctas) * 4 * rows * a.d;
+  f.pre = reinterpret_cast<int*>(p.pml + static_cast<int64_t>(ctas) * 4 * rows * 2);
   f.q = static_cast<const __nv_bfloat16*>(a.q); f.q_ld = a.q_ld;
   const bool f8 = a.k_scale != nullptr;
   int r;

@@ -13,17 +13,21 @@
 // exponents go into the weights, fp16 too: w = p 2^(E - Eref + 4) with a reference Eref at least E - 3, at most 2^15.  fp16 keeps 11
 // bits of weights down to 2^-18 of the largest, and is off by 2^-29 of it below, where a row of bf16 weights keeps 8 bits.
 //
-// The key tiles of all sequences and key heads form one line, of which every CTA (one per SM) takes an equal piece: the kernel ends
+// The key tiles of all sequences and key heads form one line, which is cut into equal pieces, two for every SM: the kernel ends
 // everywhere at the same time whatever the lengths are, and nothing but the lengths on the device decides.  A (sequence, head) that
-// lies in one piece is finished there; one that is cut leaves its unnormalised sums, at most two such parts a CTA, to a
-// second kernel.  Barriers and rings run on across items, so that the copies never stop.  Warps:
-//   0..3, 4..7  softmax of every other tile: thread t owns key t of a tile (TMEM lane t of S^T); the group's reference maximum of a
-//               row is shared and moves in large steps, and the group meets at one vote a tile on whether it has to.  The groups
-//               have sums of their own, joined at the end of an item, where a thread owns output dimension t
-//   8, 9        one lane issues S^T (a buffer for each group), one the product with the values
-//   10          TMA: a stage holds a tile of keys and values (and, of 8-bit pages, their exponent bytes)
-//   11          rows of the next item's queries
-//   12..        (8-bit pages) values to bf16, two buffers
+// lies in one piece is finished there; one that is cut leaves its unnormalised sums, at most two such parts a piece, to a
+// second kernel.  A CTA works on its two pieces tile by tile in turn, with a group of softmax warps for each, so that the
+// copies go on while one of them ends an item.  Warps:
+//   0..3, 4..7  softmax of a piece: thread t owns key t of a tile (TMEM lane t of S^T) and output dimension t; a row's reference
+//               maximum is shared and moves in large steps, and the group meets at one vote a tile on whether it has to
+//   8           one lane issues the products: of a tile with the values, then the scores of the piece's next tile
+//   9           rows of the next items' queries
+//   10, 11      TMA, a piece each: a stage holds a tile of keys and values (and, of 8-bit pages, their exponent bytes), and what the
+//               other warps have to know of it
+//   12..15      (8-bit pages) values to fp16
+// Only warps 9 to 11 walk the line, and the loops of the others are short: 16 warps in six roles share an instruction cache.  With a
+// walk of both pieces in each of them a third of all stalls was for instructions and an 8-bit tile took 1.5 to 1.8 us; with one
+// warp that copied for both pieces, 1.2.
 #pragma once
 #include "cache_attn.cuh"
 #include "chain.cuh"
@@ -35,11 +39,12 @@ struct CacheFewParams {
   const __nv_bfloat16* q;
   int64_t q_ld;
   const uint8_t *ks, *vs;
-  CacheAttnParams a;                 // po, pml: [CTA][2][R][D] and [CTA][2][R][2]
+  CacheAttnParams a;                 // po, pml: [piece][2][R][D] and [piece][2][R][2]
   int* pre;                          // [batch + 1] tiles in front of every sequence, for the second kernel
 };
 constexpr int kFewSequences = 512;   // of one launch
-constexpr int kFewLeast = 2;         // tiles of a piece: below, more CTAs cost more than they save
+constexpr int kFewLeast = 2;         // tiles of a piece where SMs have one: below, more pieces cost more than they save
+constexpr int kFewTwo = 4;           // tiles of a piece from which SMs have two
 
 template <int D, bool F8, int R>
 struct CacheFew {
@@ -52,21 +57,27 @@ struct CacheFew {
   static constexpr int kQ = 2 * kN * D;                              // bf16 rows, or two rows of codes
   static constexpr int kP = kN * kCaTile * 2;
   static constexpr int kWide = F8 ? kCaTile * D * 2 : 0;             // values in fp16
-  static constexpr int kQBufs = kN == 16 ? 2 : 1;                    // what more would take a stage away
-  static constexpr int kFixed = kQBufs * kQ + 2 * (kP + kWide);
-  static constexpr int kRest = 256 + 4 * 2 * kCaTile + 16 * kN * 4 + 64 + 13 * kFewSequences + 64;   // barriers, exponent bytes, tables
+  static constexpr int kFixed = 2 * (kQ + kP + kWide);               // each of the two pieces has its own
+  static constexpr int kRest = 256 + 4 * (2 * kCaTile + 32) + 22 * kN * 4 + 128 + 13 * kFewSequences + 64;   // barriers, exponent bytes, tables
   static constexpr int kMost = (227 * 1024 - 1024 - kRest - kFixed) / kStage;
   static constexpr int kStages = kMost < 4 ? kMost : 4;
+  // 8-bit stages are given back as soon as their keys are multiplied and the rest is read, where a piece's tiles keep to stages of
+  // their own (an even number); else, in the order of the ring, by the product with the values.  A copying warp that waits for a
+  // stage must not see it given back a turn too early.
+  static constexpr bool kEarly = F8 && kStages % 2 == 0;
   static constexpr int kTotal = kFixed + kStages * kStage + kRest + 1024;
   static constexpr uint32_t kSCols = F8 ? 2 * kN : kN;               // columns of a score buffer
-  static constexpr uint32_t kUsed = 2 * kSCols + 4 * kN;             // and two sums for each group
-  static constexpr uint32_t kCols = kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;
+  static constexpr uint32_t kUsed = 2 * kSCols + 2 * kN;             // scores and sums of two pieces
+  static constexpr uint32_t kCols = kUsed <= 64 ? 64 : kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;
   static_assert(kStages >= 2 && kTotal <= 227 * 1024 && kUsed <= 512, "room");
 };
 static_assert(2 * 168 + 2 * 88 == 4 * 128 && 2 * 208 + 88 == 3 * 168, "register shares");
 
-// Tiles of the line in front of CTA c of n; `all` < 2^31.
+// Places of the line in front of piece c of n.
 __device__ __forceinline__ int few_cut(int all, int c, int n) { return static_cast<int>(static_cast<int64_t>(all) * c / n); }
+__device__ __forceinline__ int few_pieces(int all, int ctas) {
+  return all >= 2 * kFewTwo * ctas ? 2 * ctas : max(1, min(ctas, all / kFewLeast));
+}
 
 // What the roles know of the sequences, in shared memory.
 struct CacheFewTable {
@@ -74,16 +85,17 @@ struct CacheFewTable {
   uint8_t* q_len;
 };
 
-// A role's walk along the CTA's piece [at, end) of the line: sequence by sequence, head by head.
+// A walk along a piece [at, end) of the line: sequence by sequence, head by head.  A sequence whose tokens see nothing has one
+// tile, of which nothing is seen.
 struct CacheFewItem : CacheTiles {
   int at, start, end;                // place on the line; first and last place of the piece
   int b, kvh, q_begin, q_len, shift, n;
-  int slot;                          // -1: whole, else which of the CTA's parts
+  int slot;                          // -1: whole, else which of the piece's parts
 
-  __device__ __forceinline__ void begin_walk(const CacheAttnParams& p, const CacheFewTable& t, int pieces) {
+  __device__ __forceinline__ void begin_walk(const CacheAttnParams& p, const CacheFewTable& t, int pieces, int piece) {
     const int all = t.pre[p.batch] * p.hk;
-    start = at = few_cut(all, blockIdx.x, pieces);
-    end = static_cast<int>(blockIdx.x) < pieces ? few_cut(all, blockIdx.x + 1, pieces) : at;
+    start = at = few_cut(all, min(piece, pieces), pieces);
+    end = few_cut(all, min(piece + 1, pieces), pieces);
     int low = 0, high = p.batch;     // the last sequence with pre <= at / hk
     while (high - low > 1) {
       const int mid = (low + high) / 2;
@@ -96,18 +108,52 @@ struct CacheFewItem : CacheTiles {
     while (at >= t.pre[b + 1] * p.hk) ++b;
     const int tiles = t.pre[b + 1] - t.pre[b], place = at - t.pre[b] * p.hk;
     kvh = place / tiles;
-    const int from = place - kvh * tiles, count = min(tiles - from, end - at);
-    slot = count == tiles ? -1 : at == start ? 0 : 1;
-    at += count;
+    const int from = place - kvh * tiles;
+    n = min(tiles - from, end - at);
+    slot = n == tiles ? -1 : at == start ? 0 : 1;
+    at += n;
     q_begin = t.q0[b];
     q_len = t.q_len[b];
     shift = t.len[b] - q_len;
-    n = set(shift, q_len - 1 + shift, p.window, p.first, 0, 1);
+    set(shift, q_len - 1 + shift, p.window, p.first, 0, 1);
     begin = from;
-    if (n > 0) n = count;            // a sequence that sees nothing has one place on the line
     return true;
   }
 };
+
+// What a copying warp says of the tile in a stage.
+struct alignas(16) CacheFewTile {
+  int key, flags, lo, last, first_end, pad[3];
+  __device__ __forceinline__ bool seen(int k) const { return k <= last && (k >= lo || k < first_end); }
+};
+enum : int {
+  kFewGroup = 1,                     // the piece
+  kFewFirst = 2, kFewLast = 4,       // of its item
+  kFewWhole = 8,                     // some row sees each key
+  kFewAll = 16,                      // every row sees every key
+};
+
+// A wait of few instructions (they are inlined in many places); the same limit as mbar_wait's.
+__device__ __forceinline__ bool few_wait(uint64_t* bar, uint32_t parity, uint32_t* status) {
+  uint64_t t0 = 0;
+  for (uint32_t i = 0; !mbar_try_wait(bar, parity); ++i) {
+    if ((i & 0xFFu) != 0u) continue;
+    const uint64_t now = globaltimer_ns();
+    if (i == 0) t0 = now;
+    else if (gave_up(status)) return false;
+    else if (now - t0 > YV_WAIT_LIMIT_NS) {
+      if (status != nullptr) atomicOr(status, kStatusWaitTimeout);
+      return false;
+    }
+  }
+  return true;
+}
+__device__ __forceinline__ bool few_wait_warp(uint64_t* bar, uint32_t parity, uint32_t* status) {
+  return __all_sync(0xFFFFFFFFu, few_wait(bar, parity, status)) != 0;
+}
+
+// Place in the ring of tile k of a piece: the pieces take stages in turn, as long as both have tiles.
+__device__ __forceinline__ uint32_t few_turn(uint32_t k, uint32_t group, uint32_t others) { return k + min(k + group, others); }
 
 // Descriptor of a swizzled operand: rows of `bytes` 32, 64 or 128, groups of 8 rows one after the other (modes 6, 4, 2).  K-major
 // rows hold consecutive k, MN-major ones consecutive columns of one k.  Within a row the 16-byte places are exchanged by the
@@ -126,8 +172,6 @@ template <int BYTES>
 __device__ __forceinline__ int few_place(int row, int place) {
   return BYTES == 128 ? place ^ (row & 7) : BYTES == 64 ? place ^ ((row >> 1) & 3) : place ^ ((row >> 2) & 1);
 }
-
-__device__ __forceinline__ int few_pieces(int tiles, int ctas) { return max(1, min(ctas, tiles / kFewLeast)); }
 
 // 8 e4m3 codes -> 8 fp16 numbers, exactly
 __device__ __forceinline__ uint4 few_halves(uint32_t a, uint32_t b) {
@@ -193,26 +237,29 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
   uint8_t* sWide = smem;                                             // [2]
   uint8_t* sRing = sWide + 2 * S::kWide;
   uint8_t* sP = sRing + kStages * S::kStage;                         // [2]
-  uint8_t* sQ = sP + 2 * S::kP;                                      // [kQBufs]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sQ + S::kQBufs * S::kQ);
+  uint8_t* sQ = sP + 2 * S::kP;                                      // [2]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sQ + 2 * S::kQ);
   uint64_t* full = bars;                     // [kStages] keys, values and exponent bytes have landed
   uint64_t* empty = bars + kStages;          // [kStages]
+  // of a piece:
   uint64_t* s_full = bars + 2 * kStages;     // [2]
   uint64_t* p_full = s_full + 2;             // [2] weights are stored and all scores read
   uint64_t* pv_done = p_full + 2;            // [2]
   uint64_t* v_full = pv_done + 2;            // [2] widened values
-  uint64_t* q_full = v_full + 2;             // [2] query rows and their tables
-  uint64_t* t_empty = q_full + 2;            // [2] tables
-  uint64_t* o_empty = t_empty + 2;           // [2]
-  uint64_t* q_empty = o_empty + 2;           // [kQBufs] query rows
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_empty + 2);
+  uint64_t* q_empty = v_full + 2;            // [2] query rows
+  uint64_t* q_full = q_empty + 2;            // [2][2] query rows and their tables, of which there are two
+  uint64_t* t_empty = q_full + 4;            // [2][2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(t_empty + 4);
   uint8_t* sByte = reinterpret_cast<uint8_t*>(bars) + 256;                               // [kStages][2][128]
-  int* sHi = reinterpret_cast<int*>(sByte + kStages * 2 * kCaTile);                      // [2][N] last visible key of a row, -1 = none
-  int* sRow = sHi + 2 * N;                                                               // [2][N] token << 8 | head of the group
-  float* sFactor = reinterpret_cast<float*>(sRow + 2 * N);                               // [2][N] a row's power of two times the scale
-  float* sM = sFactor + 2 * N;                                                           // [2 groups][N] reference maxima
-  float* sRed = sM + 2 * N;                                                              // [2 groups][4][N]; a new maximum goes to [0]
-  int* sTop = reinterpret_cast<int*>(sRed + 8 * N);                                      // [2 groups][8] largest exponent bytes, reference
+  CacheFewTile* sTile = reinterpret_cast<CacheFewTile*>(sByte + kStages * 2 * kCaTile);  // [kStages]
+  volatile int* sFirst = reinterpret_cast<int*>(bars) + 60;                              // [2] whether the weights are an item's first
+  int4* sItem = reinterpret_cast<int4*>(sTile + kStages);                                // [2][2] first row of q, key head, slot
+  int* sHi = reinterpret_cast<int*>(sItem + 4);                    // [2][2][N] last visible key of a row, -1 = none
+  int* sRow = sHi + 4 * N;                                                               // [2][2][N] token << 8 | head of the group
+  float* sFactor = reinterpret_cast<float*>(sRow + 4 * N);                               // [2][2][N] a row's power of two times the scale
+  float* sM = sFactor + 4 * N;                                                           // [2][N] reference maxima
+  float* sRed = sM + 2 * N;                                                              // [2][4][N]; a new maximum goes to [0]
+  int* sTop = reinterpret_cast<int*>(sRed + 8 * N);                                      // [2][8] largest exponent bytes, reference
   CacheFewTable tab;
   tab.pre = sTop + 16;
   tab.q0 = tab.pre + kFewSequences + 1;
@@ -226,17 +273,18 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
     tma_prefetch_desc(&fp.tma_v);
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], F8 ? 9 : 1);      // 8 bits: the score product, four softmax warps, four widening ones; else the P V product
+      mbar_init(&empty[s], S::kEarly ? 9 : 1);         // early: the score product, four softmax warps, four widening ones
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
       mbar_init(&pv_done[i], 1);
       mbar_init(&v_full[i], 4);
-      mbar_init(&q_full[i], 1);
-      mbar_init(&t_empty[i], 8);
       mbar_init(&q_empty[i], 1);
-      mbar_init(&o_empty[i], 8);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&t_empty[i], 4);
     }
     fence_barrier_init();
   }
@@ -249,7 +297,7 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
   // query rows that do not exist stay zero
-  for (int i = tid; i < S::kQBufs * S::kQ / 16; i += S::kThreads) reinterpret_cast<uint4*>(sQ)[i] = make_uint4(0, 0, 0, 0);
+  for (int i = tid; i < 2 * S::kQ / 16; i += S::kThreads) reinterpret_cast<uint4*>(sQ)[i] = make_uint4(0, 0, 0, 0);
   fence_proxy_async_smem();
   // the tensor memory is this kernel's before the next one may begin
   chain_next();
@@ -299,43 +347,63 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
 
   auto stage_v = [&](uint32_t s) { return sRing + s * S::kStage; };
   auto stage_k = [&](uint32_t s) { return sRing + s * S::kStage + S::kHalf; };
-  const uint32_t tO = tmem_base + 2 * S::kSCols;                     // [2 items][2 groups] of N columns behind the scores
+  const uint32_t tO = tmem_base + 2 * S::kSCols;                     // [2] of N columns behind the scores
+
+  // tiles of both pieces
+  const int places = tab.pre[p.batch] * p.hk;
+  auto tiles_of = [&](int piece) { return few_cut(places, min(piece + 1, pieces), pieces) - few_cut(places, min(piece, pieces), pieces); };
+  // the longer one is the first
+  const int extra = tiles_of(gridDim.x + blockIdx.x) > tiles_of(blockIdx.x) ? 1 : 0;
+  auto piece_of = [&](uint32_t group) { return static_cast<int>(blockIdx.x + ((group ^ extra) != 0u ? gridDim.x : 0u)); };
+  const int both = tiles_of(piece_of(0)) + tiles_of(piece_of(1));
 
   if (kShares && warp >= 8) regs_give<S::kOtherRegs>();
-  if (warp == 10) {
+  if (warp == 10 || warp == 11) {
     // ------------------------------------ copies --------------------------------------------
-    const uint32_t lead = elect_one() ? 1u : 0u;
-    const int boxes = kCaTile / p.box, per_look = 32 / boxes;
-    uint32_t g = 0;                                                  // tiles so far
+    const uint32_t grp = warp - 10, lead = elect_one() ? 1u : 0u;
+    const int piece = piece_of(grp), boxes = kCaTile / p.box, per_look = 32 / boxes;
+    const uint32_t others = both - tiles_of(piece);
+    uint32_t k = 0;
     bool ok = true;
     CacheFewItem it;
-    it.begin_walk(p, tab, pieces);
+    it.begin_walk(p, tab, pieces, piece);
     while (ok && it.next(p, tab)) {
-      // slot of copy `lane` of the tiles from j0 on, and its place in the page; negative where no key of it is seen
-      auto look = [&](int j0) {
-        const int j = j0 + lane / boxes, key = it.first_key(j) + (lane % boxes) * p.box;
-        return j < it.n && it.any(key, p.box) ? make_int2(ca_slot(p, it.b, key), key % p.block) : make_int2(-1, 0);
-      };
-      int2 rows = look(0), next = make_int2(-1, 0);
-      for (int j = 0, in = 0; j < it.n && ok; ++j, ++g) {
-        if (in == 0) {
-          if (j > 0) rows = next;
-          next = look(j + per_look);
+      int2 rows = {}, next = {};
+      for (int j = 0, in = per_look; j < it.n; ++j, ++k) {
+        // lane i: slot of copy i of the next tiles and its place in the page (negative where no key of it is seen), looked up ahead
+        for (; in == per_look; in = 0) {
+          for (int ahead = j == 0 ? 0 : per_look; ahead <= per_look; ahead += per_look) {
+            const int at = j + ahead + lane / boxes, key = it.first_key(at) + (lane % boxes) * p.box;
+            rows = next;
+            next = at < it.n && it.any(key, p.box) ? make_int2(ca_slot(p, it.b, key), key % p.block) : make_int2(-1, 0);
+          }
         }
-        const uint32_t s = g % kStages;
+        const uint32_t g = few_turn(k, grp, others), s = g % kStages;
         const uint32_t here = __ballot_sync(0xFFFFFFFFu, rows.x >= 0 && lane / boxes == in);
-        ok = mbar_wait_warp(&empty[s], ((g / kStages) & 1u) ^ 1u, p.status);
+        ok = few_wait_warp(&empty[s], ((g / kStages) & 1u) ^ 1u, p.status);
         if (!ok) break;
-        if (lead) mbar_expect_tx(&full[s], static_cast<uint32_t>(__popc(here)) * p.box * (F8 ? 2 * D + 2 : 4 * D));
+        if (lead) {
+          const int key0 = it.first_key(j);
+          const bool whole = it.whole(key0);
+          const bool all = whole && key0 + kCaTile - 1 <= it.shift &&
+                           (p.window == 0 || key0 > it.q_len - 1 + it.shift - p.window || key0 + kCaTile <= p.first);
+          sTile[s].key = key0;
+          sTile[s].flags = static_cast<int>(grp) | (j == 0 ? kFewFirst : 0) | (j + 1 == it.n ? kFewLast : 0) | (whole ? kFewWhole : 0) |
+                           (all ? kFewAll : 0);
+          sTile[s].lo = it.lo;
+          sTile[s].last = it.last;
+          sTile[s].first_end = it.first_end;
+          mbar_expect_tx(&full[s], static_cast<uint32_t>(__popc(here)) * p.box * (F8 ? 2 * D + 2 : 4 * D));
+        }
         for (int i = 0; i < boxes; ++i) {
           const int row = __shfl_sync(0xFFFFFFFFu, rows.x, in * boxes + i), off = __shfl_sync(0xFFFFFFFFu, rows.y, in * boxes + i);
           if (!lead || row < 0) continue;
           if constexpr (F8) {
-            const int64_t at = static_cast<int64_t>(row) * p.hk + it.kvh * p.block - off * (p.hk - 1);     // [page][head][place]
+            const int64_t from = static_cast<int64_t>(row) * p.hk + it.kvh * p.block - off * (p.hk - 1);   // [page][head][place]
             tma_load_3d(stage_k(s) + i * p.box * D, &fp.tma_k, &full[s], 0, it.kvh, row);
-            bulk_load_1d(sByte + s * 2 * kCaTile + i * p.box, fp.ks + at, p.box, &full[s]);
+            bulk_load_1d(sByte + s * 2 * kCaTile + i * p.box, fp.ks + from, p.box, &full[s]);
             tma_load_3d(stage_v(s) + i * p.box * D, &fp.tma_v, &full[s], 0, it.kvh, row);
-            bulk_load_1d(sByte + s * 2 * kCaTile + kCaTile + i * p.box, fp.vs + at, p.box, &full[s]);
+            bulk_load_1d(sByte + s * 2 * kCaTile + kCaTile + i * p.box, fp.vs + from, p.box, &full[s]);
           } else {
 #pragma unroll
             for (int c = 0; c < D / 64; ++c) tma_load_3d(stage_k(s) + c * kSlab + i * p.box * 128, &fp.tma_k, &full[s], c * 64, it.kvh, row);
@@ -344,24 +412,36 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
           }
         }
         __syncwarp();
-        in = in + 1 == per_look ? 0 : in + 1;
+        ++in;
       }
     }
-  } else if (warp == 11) {
+  } else if (warp == 9) {
     // ------------------------------------ query rows ----------------------------------------
-    uint32_t items = 0;
-    bool ok = true;
-    CacheFewItem it;
-    it.begin_walk(p, tab, pieces);
-    while (ok && it.next(p, tab)) {
-      if (it.n == 0) continue;
-      const uint32_t tb = items & 1u, qb = items % S::kQBufs;
-      ok = mbar_wait_warp(&q_empty[qb], ((items / S::kQBufs) & 1u) ^ 1u, p.status) &&
-           mbar_wait_warp(&t_empty[tb], ((items >> 1) & 1u) ^ 1u, p.status);
-      if (!ok) break;
-      ++items;
+    // Items of both pieces, in the order in which their first tiles are multiplied.
+    const int n0 = tiles_of(piece_of(0));
+    uint32_t items[2] = {0u, 0u}, k[2] = {0u, 0u};                   // items and tiles so far
+    CacheFewItem now, then;
+    uint32_t grp = 0;
+    now.begin_walk(p, tab, pieces, piece_of(0));
+    then.begin_walk(p, tab, pieces, piece_of(1));
+    for (;;) {
+      const uint32_t turn0 = few_turn(k[0], 0, both - n0), turn1 = few_turn(k[1], 1, n0);
+      const bool live0 = k[0] < static_cast<uint32_t>(n0), live1 = k[1] < static_cast<uint32_t>(both - n0);
+      if (!live0 && !live1) break;
+      const uint32_t want = !live0 || (live1 && turn1 < turn0) ? 1u : 0u;
+      if (want != grp) {
+        const CacheFewItem other = then;
+        then = now;
+        now = other;
+        grp = want;
+      }
+      CacheFewItem& it = now;
+      it.next(p, tab);
+      const uint32_t item = grp != 0 ? items[1] : items[0], tb = grp * 2 + (item & 1u);
+      if (!few_wait_warp(&q_empty[grp], (item & 1u) ^ 1u, p.status) || !few_wait_warp(&t_empty[tb], ((item >> 1) & 1u) ^ 1u, p.status)) break;
+      if (lane == 0) sItem[tb] = make_int4(it.q_begin, it.kvh, it.slot, 0);
       constexpr int E = D / 32;                                      // numbers of a lane
-      uint8_t* dst = sQ + qb * S::kQ;
+      uint8_t* dst = sQ + grp * S::kQ;
       constexpr int kAhead = R < 16 ? R : 16;                        // rows whose loads are under way together
 #pragma unroll 1
       for (int i0 = 0; i0 < R; i0 += kAhead) {
@@ -439,74 +519,70 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_full[tb]);
+      if (grp != 0) { ++items[1]; k[1] += it.n; } else { ++items[0]; k[0] += it.n; }
     }
   } else if (warp == 8) {
-    // ------------------------------------ scores --------------------------------------------
+    // ------------------------------------ products ------------------------------------------
     if (elect_one()) {
-      uint32_t g = 0, items = 0;
-      bool ok = true;
-      CacheFewItem it;
-      it.begin_walk(p, tab, pieces);
-      while (ok && it.next(p, tab)) {
-        if (it.n == 0) continue;
-        const uint32_t qb = items % S::kQBufs;
-        ok = mbar_wait(&q_full[items & 1u], (items >> 1) & 1u, p.status);
-        ++items;
-        const uint32_t aQ = smem_u32(sQ + qb * S::kQ);
-        for (int j = 0; j < it.n && ok; ++j, ++g) {
-          const uint32_t s = g % kStages, sb = g & 1u;
-          // the buffer's scores, of tile g - 2, have been read
-          ok = mbar_wait(&full[s], (g / kStages) & 1u, p.status) && (g < 2 || mbar_wait(&p_full[sb], ((g >> 1) & 1u) ^ 1u, p.status));
-          if (!ok) break;
-          tc_fence_after_sync();
-          const uint32_t aK = smem_u32(stage_k(s)), tS = tmem_base + sb * S::kSCols;
-          if constexpr (F8) {
+      const uint32_t n0 = tiles_of(piece_of(0)), n1 = both - n0;
+      uint32_t items0 = 0, items1 = 0;
+      // scores of tile k of a piece
+      auto scores = [&](uint32_t i, uint32_t k) -> bool {
+        const uint32_t g = few_turn(k, i, i != 0 ? n0 : n1), s = g % kStages;
+        if (!few_wait(&full[s], (g / kStages) & 1u, p.status)) return false;
+        const int flags = sTile[s].flags;
+        const uint32_t item = i != 0 ? items1 : items0;
+        if ((flags & kFewFirst) != 0 && !few_wait(&q_full[i * 2 + (item & 1u)], (item >> 1) & 1u, p.status)) return false;
+        tc_fence_after_sync();
+        const uint32_t aK = smem_u32(stage_k(s)), aQ = smem_u32(sQ + i * S::kQ), tS = tmem_base + i * S::kSCols;
+        if constexpr (F8) {
 #pragma unroll
-            for (int kk = 0; kk < D / 32; ++kk)
-              tc_mma_f8_ss(tS, few_desc<D>(aK + kk * 32), few_desc<D>(aQ + kk * 32), kIdescS, kk != 0 ? 1u : 0u);
-          } else {
+          for (int kk = 0; kk < D / 32; ++kk)
+            tc_mma_f8_ss(tS, few_desc<D>(aK + kk * 32), few_desc<D>(aQ + kk * 32), kIdescS, kk != 0 ? 1u : 0u);
+        } else {
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk)
-              tc_mma_f16_ss(tS, few_desc<128>(aK + (kk / 4) * kSlab + (kk % 4) * 32), few_desc<128>(aQ + (kk / 4) * (N * 128) + (kk % 4) * 32),
-                            kIdescS, kk != 0 ? 1u : 0u);
-          }
-          tc_commit(&s_full[sb]);
-          if (F8) tc_commit(&empty[s]);
-          if (j + 1 == it.n) tc_commit(&q_empty[qb]);
+          for (int kk = 0; kk < D / 16; ++kk)
+            tc_mma_f16_ss(tS, few_desc<128>(aK + (kk / 4) * kSlab + (kk % 4) * 32), few_desc<128>(aQ + (kk / 4) * (N * 128) + (kk % 4) * 32),
+                          kIdescS, kk != 0 ? 1u : 0u);
         }
-      }
-    }
-  } else if (warp == 9) {
-    // ------------------------------------ weights times values ------------------------------
-    if (elect_one()) {
-      uint32_t g = 0, items = 0;
-      bool ok = true;
-      CacheFewItem it;
-      it.begin_walk(p, tab, pieces);
-      while (ok && it.next(p, tab)) {
-        if (it.n == 0) continue;
-        const uint32_t ob = items & 1u;
-        ok = mbar_wait(&o_empty[ob], ((items >> 1) & 1u) ^ 1u, p.status);
-        ++items;
-        for (int j = 0; j < it.n && ok; ++j, ++g) {
-          const uint32_t s = g % kStages, pb = g & 1u, ph = (g >> 1) & 1u;
-          ok = (F8 ? mbar_wait(&v_full[pb], ph, p.status) : mbar_wait(&full[s], (g / kStages) & 1u, p.status)) &&
-               mbar_wait(&p_full[pb], ph, p.status);
-          if (!ok) break;
+        tc_commit(&s_full[i]);
+        if (S::kEarly) tc_commit(&empty[s]);
+        if ((flags & kFewLast) != 0) {
+          tc_commit(&q_empty[i]);
+          if (i != 0) ++items1; else ++items0;
+        }
+        return true;
+      };
+      uint32_t k0 = 0, k1 = 0;                                       // tiles of the pieces
+      // the first scores of both, then tile by tile in the order of the ring; a lone call of `scores`, so that its code is there once
+      for (int g = -2; g < both; ++g) {
+        uint32_t i, next;
+        if (g < 0) {
+          i = g + 2;
+          next = 0;
+        } else {
+          i = k0 >= n0 || (k1 < n1 && k1 < k0) ? 1u : 0u;
+          const uint32_t k = i != 0 ? k1 : k0, at = few_turn(k, i, i != 0 ? n0 : n1), s = at % kStages;
+          // the weights are stored and the scores read; of 8 bits the stage may be another tile's by now
+          if (!few_wait(&p_full[i], k & 1u, p.status) || (F8 && !few_wait(&v_full[i], k & 1u, p.status))) break;
           tc_fence_after_sync();
-          const uint32_t aV = F8 ? smem_u32(sWide + pb * S::kWide) : smem_u32(stage_v(s)), aP = smem_u32(sP + pb * S::kP);
+          const uint32_t aV = F8 ? smem_u32(sWide + i * S::kWide) : smem_u32(stage_v(s)), aP = smem_u32(sP + i * S::kP);
+          const uint32_t more = sFirst[i] == 0 ? 1u : 0u;
 #pragma unroll
           for (int kk = 0; kk < kCaTile / 16; ++kk)
-            tc_mma_f16_ss(tO + (ob * 2 + pb) * N, make_smem_desc(aV + kk * 2048, kSlab, 1024), few_desc<kPRow>(aP + kk * 16 * kPRow), kIdescPV,
-                          j >= 2 || kk != 0 ? 1u : 0u);
-          tc_commit(&pv_done[pb]);
-          if (!F8) tc_commit(&empty[s]);
+            tc_mma_f16_ss(tO + i * N, make_smem_desc(aV + kk * 2048, kSlab, 1024), few_desc<kPRow>(aP + kk * 16 * kPRow), kIdescPV,
+                          kk != 0 ? 1u : more);
+          tc_commit(&pv_done[i]);
+          if (!S::kEarly) tc_commit(&empty[s]);
+          next = k + 1;
+          if (i != 0) ++k1; else ++k0;
         }
+        if (next < (i != 0 ? n1 : n0) && !scores(i, next)) break;
       }
     }
   } else if (warp >= 12) {
     if constexpr (F8) {
-    // ------------------------------------ values to fp16 ------------------------------------
+      // ------------------------------------ values to fp16 ----------------------------------
     constexpr int kLanes = D / 16;                                   // lanes of a row, 16 codes each
     constexpr int kStep = 128 / kLanes, kRows = kCaTile / kStep;
     const int c = (tid - 384) % kLanes, row0 = (tid - 384) / kLanes;
@@ -515,30 +591,26 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
     const int w = (2 * c) & 7, odd_first = D == 128 && c >= 4 ? 1 : 0;
     const uint32_t place0 = (c / 4) * kSlab + row0 * 128 + (((w + odd_first) ^ (row0 & 7)) << 4);
     const uint32_t place1 = (c / 4) * kSlab + row0 * 128 + (((w + 1 - odd_first) ^ (row0 & 7)) << 4);
-    uint32_t g = 0;
-    bool ok = true;
-    CacheFewItem it;
-    it.begin_walk(p, tab, pieces);
-    while (ok && it.next(p, tab)) {
-      for (int j = 0; j < it.n && ok; ++j, ++g) {
-        const uint32_t s = g % kStages, vb = g & 1u;
-        const int key0 = it.first_key(j);
-        ok = mbar_wait_warp(&full[s], (g / kStages) & 1u, p.status);
-        if (!ok) break;
+      uint32_t k0 = 0, k1 = 0, s = 0, ph = 0;                        // tiles of the pieces
+      for (int g = 0; g < both; ++g) {
+        if (!few_wait_warp(&full[s], ph, p.status)) break;
         const uint8_t* src = stage_v(s) + row0 * D + c * 16;
         uint4 x[kRows];
 #pragma unroll
         for (int i = 0; i < kRows; ++i) x[i] = *reinterpret_cast<const uint4*>(src + i * kStep * D);
-        if (!it.whole(key0)) {                                       // values that no row sees are cleared (0 * NaN would be NaN)
+        const int flags = sTile[s].flags;
+        if ((flags & kFewWhole) == 0) {                              // values that no row sees are cleared (0 * NaN would be NaN)
+          const CacheFewTile tile = sTile[s];
 #pragma unroll
           for (int i = 0; i < kRows; ++i)
-            if (!it.seen(key0 + row0 + i * kStep)) x[i] = make_uint4(0, 0, 0, 0);
+            if (!tile.seen(tile.key + row0 + i * kStep)) x[i] = make_uint4(0, 0, 0, 0);
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[s]);
-        ok = g < 2 || mbar_wait_warp(&pv_done[vb], ((g >> 1) & 1u) ^ 1u, p.status);
-        if (!ok) break;
-        uint8_t* dst = sWide + vb * S::kWide;
+        if (S::kEarly && lane == 0) mbar_arrive(&empty[s]);
+        const bool second = (flags & kFewGroup) != 0;
+        const uint32_t i_side = second ? 1u : 0u, mine = second ? k1 : k0;
+        if (mine > 0 && !few_wait_warp(&pv_done[i_side], (mine - 1) & 1u, p.status)) break;
+        uint8_t* dst = sWide + i_side * S::kWide;
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
           const uint4 a = few_halves(x[i].x, x[i].y), b = few_halves(x[i].z, x[i].w);
@@ -547,52 +619,44 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&v_full[vb]);
+        if (lane == 0) mbar_arrive(&v_full[i_side]);
+        if (second) ++k1; else ++k0;
+        if (++s == kStages) { s = 0; ph ^= 1u; }
       }
-    }
     }
   } else if (warp < 8) {
     // ------------------------------------ softmax -------------------------------------------
     if constexpr (kShares) regs_take<S::kSoftmaxRegs>();
-    const uint32_t grp = warp >> 2;                                  // tiles g with g % 2 == grp
+    const uint32_t grp = warp >> 2;                                  // the piece of this warp
     const int t = tid & 127, bar = 1 + grp;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t tS = tmem_base + lane_off + grp * S::kSCols;
+    const uint32_t tS = tmem_base + lane_off + grp * S::kSCols, to = tO + lane_off + grp * N;
     float *m_mine = sM + grp * N, *red = sRed + grp * 4 * N;
     int* top = sTop + grp * 8;                                       // [0..3] of the warps, [7] the reference byte
     uint8_t* sp = sP + grp * S::kP + t * kPRow;
-    uint32_t g0 = 0, items = 0;
+    uint32_t k = 0, items = 0;                                       // tiles and items so far
     bool ok = true;
-    CacheFewItem it;
-    it.begin_walk(p, tab, pieces);
-    while (it.next(p, tab)) {
-      const uint32_t tb = items & 1u, ob = items & 1u;
-      const int first = (g0 & 1u) == grp ? 0 : 1;                    // first tile of this group; how many it and the other have
-      const int mine = (it.n - first + 1) / 2;
-      float l[R];
+    const int piece = piece_of(grp);
+    const uint32_t mine = tiles_of(piece), others = both - mine;
+    float l[R];
+    for (; k < mine; ++k) {
+      const uint32_t g = few_turn(k, grp, others), s = g % kStages, ph = k & 1u;
+      const uint32_t tb = grp * 2 + (items & 1u);
+      // a warp whose wait ran out (what it reads of the tile may then be anything) goes to the vote; the group leaves there together
+      ok = ok && few_wait(&full[s], (g / kStages) & 1u, p.status);
+      const int flags = sTile[s].flags, key = sTile[s].key + t;
+      const bool first = (flags & kFewFirst) != 0;                   // the group's maxima and reference are an earlier item's
+      if (first) {
 #pragma unroll
-      for (int i = 0; i < R; ++i) l[i] = 0.f;
-      if (it.n > 0) {
-        ++items;
-        if (t < R) m_mine[t] = -1.0e29f;
-        if (t == 0) top[7] = -1024;
-        ok = mbar_wait(&q_full[tb], ((items - 1) >> 1) & 1u, p.status);
-        ok = !few_any<128>(bar, !ok);                                // the maxima are set; all agree on whether a wait ran out
+        for (int i = 0; i < R; ++i) l[i] = 0.f;
+        ok = ok && few_wait(&q_full[tb], (items >> 1) & 1u, p.status);
       }
-      // rows are masked one by one only where some row does not see the whole tile
-      const int hi_least = it.shift, hi_most = it.q_len - 1 + it.shift;
-      // a warp whose wait ran out walks on, without waiting, to the next vote; the group leaves there together
-      for (int j = first; j < it.n && (ok || j > first); j += 2) {
-        const uint32_t g = g0 + j, s = g % kStages, ph = (g >> 1) & 1u;
-        const int key0 = it.first_key(j), key = key0 + t;
-        const bool seen = it.seen(key), whole = it.whole(key0);
-        const bool all = whole && key0 + kCaTile - 1 <= hi_least &&
-                         (p.window == 0 || key0 > hi_most - p.window || key0 + kCaTile <= p.first);
-        ok = ok && mbar_wait(&s_full[grp], ph, p.status);
-        if (F8 || !whole) ok = ok && mbar_wait(&full[s], (g / kStages) & 1u, p.status);
+      {
+        const bool seen = (flags & kFewWhole) != 0 || sTile[s].seen(key);
+        ok = ok && few_wait(&s_full[grp], ph, p.status);
         ok = __all_sync(0xFFFFFFFFu, ok);                            // the aligned tcgen05 instructions need a converged warp
         float sc[R];
-        bool high = false;
+        bool high = first;
         int vbyte = 0;
         if (ok) {
           tc_fence_after_sync();
@@ -600,7 +664,9 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
           if (F8) {
             kf = few_power(sByte[s * 2 * kCaTile + t]);
             vbyte = seen ? sByte[s * 2 * kCaTile + kCaTile + t] : 0;
-            high = vbyte > top[7] + 3 && vbyte != 255;               // NaN needs no reference
+            __syncwarp();
+            if (S::kEarly && lane == 0) mbar_arrive(&empty[s]);
+            high |= vbyte > top[7] + 3 && vbyte != 255;              // NaN needs no reference
           }
 #pragma unroll
           for (int n0 = 0; n0 < N; n0 += 16) {
@@ -623,7 +689,7 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
               for (int i = 0; i < kHere; ++i) sc[n0 + i] = __uint_as_float(a[i]) * kf;
             }
           }
-          if (!all) {
+          if ((flags & kFewAll) == 0) {
 #pragma unroll
             for (int i = 0; i < R; ++i) {
               const int hi = sHi[tb * N + i];
@@ -641,7 +707,7 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
         // lazy: a reference maximum moves only when a score exceeds it by more than 2^8 (or is NaN)
         const bool moves = few_any<128>(bar, high || !ok);
         // the product of the group's last tile has landed: its P buffer is free, its sums may be rescaled
-        if (g >= 2) ok = ok && mbar_wait(&pv_done[grp], ph ^ 1u, p.status);
+        if (k > 0) ok = ok && few_wait(&pv_done[grp], ph ^ 1u, p.status);
         ok = __all_sync(0xFFFFFFFFu, ok);
         if (moves) {
           if (ok) {
@@ -660,31 +726,31 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
           ok = !few_any<128>(bar, !ok);
           if (!ok) break;
           // a reference exponent that is passed by more than 3 moves as the maxima do
-          const int old_ref = F8 ? top[7] : 0, most = F8 ? max(max(top[0], top[1]), max(top[2], top[3])) : 0;
+          const int old_ref = !F8 ? 0 : first ? -1024 : top[7], most = F8 ? max(max(top[0], top[1]), max(top[2], top[3])) : 0;
           const int ref = most > old_ref + 3 ? most : old_ref;
           const float rescale = F8 ? ex2(static_cast<float>(old_ref - ref)) : 1.f;
           if (t < R) {
-            const float top = max_nan(max_nan(red[t], red[N + t]), max_nan(red[2 * N + t], red[3 * N + t]));
-            red[t] = !(top <= m_mine[t] + kCaRescale) ? top : m_mine[t];
+            const float now = max_nan(max_nan(red[t], red[N + t]), max_nan(red[2 * N + t], red[3 * N + t]));
+            const float old = first ? -1.0e29f : m_mine[t];
+            red[t] = !(now <= old + kCaRescale) ? now : old;
           }
           few_any<128>(bar, false);
           tc_fence_after_sync();
-          const uint32_t to = tO + lane_off + (ob * 2 + grp) * N;
 #pragma unroll
           for (int n0 = 0; n0 < N; n0 += 16) {
             constexpr int kHere = R < 16 ? R : 16;
             uint32_t o[16];
-            if (j > first) {
+            if (!first) {
               tmem_ld16(to + n0, o);
               tc_wait_ld();
             }
 #pragma unroll
             for (int i = 0; i < kHere; ++i) {
-              const float alpha = ex2(m_mine[n0 + i] - red[n0 + i]);
+              const float alpha = first ? 1.f : ex2(m_mine[n0 + i] - red[n0 + i]);
               l[n0 + i] *= alpha;
-              if (j > first) o[i] = __float_as_uint(__uint_as_float(o[i]) * (F8 ? alpha * rescale : alpha));
+              if (!first) o[i] = __float_as_uint(__uint_as_float(o[i]) * (F8 ? alpha * rescale : alpha));
             }
-            if (j > first) {
+            if (!first) {
               tmem_st16(to + n0, o);
               tc_wait_st();
             }
@@ -724,7 +790,7 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
             for (int i = 0; i < R / 8; ++i)
               *reinterpret_cast<uint4*>(sp + (few_place<kPRow>(t, i) << 4)) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
           }
-          if (!F8 && !whole && !seen) {              // values that no row sees are cleared (0 * NaN would be NaN)
+          if (!F8 && !seen) {              // values that no row sees are cleared (0 * NaN would be NaN)
 #pragma unroll
             for (int c = 0; c < D / 64; ++c)
 #pragma unroll
@@ -734,86 +800,51 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
           tc_fence_before_sync();
           __syncwarp();
           if (lane == 0) {
+            if ((warp & 3) == 0) sFirst[grp] = first ? 1 : 0;
             mbar_arrive(&p_full[grp]);
-            if (F8) mbar_arrive(&empty[s]);
           }
         }
       }
-      if (it.n > 0) {
-        const uint32_t end = g0 + first + 2 * mine - 2;              // this group's last tile
-        if (mine > 0) ok = ok && mbar_wait(&pv_done[grp], (end >> 1) & 1u, p.status);
+      if ((flags & kFewLast) == 0) continue;
+      // ---- the end of an item
+      ok = ok && few_wait(&pv_done[grp], ph, p.status);
 #pragma unroll
-        for (int i = 0; i < R; ++i) {
-          float v = l[i];
+      for (int i = 0; i < R; ++i) {
+        float v = l[i];
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-          if (lane == 0) red[(warp & 3) * N + i] = v;
-        }
-        ok = !few_any<256>(3, !ok);
-        if (!ok) break;                              // a wait ran out (the status word says so): the outputs are not written
-        tc_fence_after_sync();
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+        if (lane == 0) red[(warp & 3) * N + i] = v;
       }
-      // The groups' sums are joined, half of the rows by each group.  A group without a tile has the sum zero, and no product.
-      const bool has0 = it.n > 0 && (it.n > 1 || (g0 & 1u) == 0u), has1 = it.n > 0 && (it.n > 1 || (g0 & 1u) == 1u);
-      const float ref0 = F8 ? few_power(max(sTop[7], 0)) * 0.0625f : 1.f, ref1 = F8 ? few_power(max(sTop[15], 0)) * 0.0625f : 1.f;
-      constexpr int kHalfRows = R / 2, kAtOnce = kHalfRows < 16 ? kHalfRows : 16;
+      ok = !few_any<128>(bar, !ok);
+      if (!ok) break;                                // a wait ran out (the status word says so): the outputs are not written
+      tc_fence_after_sync();
+      const int4 item = sItem[tb];                   // first row of q, key head, slot
+      ++items;
+      const float back = F8 ? few_power(max(top[7], 0)) * 0.0625f : 1.f;                 // 2^(Eref - 4)
 #pragma unroll 1
-      for (int part = 0; part < kHalfRows; part += kAtOnce) {
-        const int r0 = static_cast<int>(grp) * kHalfRows + part;     // first row
-        const int n0 = r0 & ~15;
-        uint32_t o0[16], o1[16];
+      for (int n0 = 0; n0 < R; n0 += 16) {
+        constexpr int kHere = R < 16 ? R : 16;
+        uint32_t o[16];
+        tmem_ld16(to + n0, o);
+        tc_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o0[i] = o1[i] = 0u;
-        if (it.n > 0) {
-          if (has0) tmem_ld16(tO + lane_off + (ob * 2) * N + n0, o0);
-          if (has1) tmem_ld16(tO + lane_off + (ob * 2 + 1) * N + n0, o1);
-          tc_wait_ld();
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          if (kAtOnce < 16 && (i >= R || (i >= kHalfRows) != (grp != 0))) continue;
-          const int row = n0 + i;
-          int tok, h;
-          float sum = 0.f, f0 = 0.f, f1 = 0.f, m = -1.0e29f;
-          if (it.n > 0) {
-            const int at = sRow[tb * N + row];
-            if (at < 0) continue;
-            tok = at >> 8;
-            h = at & 255;
-            m = max_nan(sM[row], sM[N + row]);
-            f0 = ex2(sM[row] - m);
-            f1 = ex2(sM[N + row] - m);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) sum += sRed[q * N + row] * f0 + sRed[(4 + q) * N + row] * f1;
-            if (F8) {                                                // 2^(Eref - 4)
-              f0 *= has0 ? ref0 : 0.f;
-              f1 *= has1 ? ref1 : 0.f;
-            }
-          } else {
-            tok = row / p.group;
-            h = row - tok * p.group;
-            if (tok >= it.q_len) continue;
-          }
-          const float o = __uint_as_float(o0[i]) * f0 + __uint_as_float(o1[i]) * f1;
-          if (it.slot >= 0) {
-            const int64_t part = (static_cast<int64_t>(blockIdx.x) * 2 + it.slot) * R + row;
-            if (t < D) p.po[part * D + t] = o;
-            if (t == 0) *reinterpret_cast<float2*>(p.pml + part * 2) = make_float2(m, sum);
+        for (int i = 0; i < kHere; ++i) {
+          const int row = n0 + i, at = sRow[tb * N + row];
+          if (at < 0) continue;
+          const float sum = (red[row] + red[N + row]) + (red[2 * N + row] + red[3 * N + row]), v = __uint_as_float(o[i]) * back;
+          if (item.z >= 0) {
+            const int64_t part = (static_cast<int64_t>(piece) * 2 + item.z) * R + row;
+            if (t < D) p.po[part * D + t] = v;
+            if (t == 0) *reinterpret_cast<float2*>(p.pml + part * 2) = make_float2(m_mine[row], sum);
           } else if (t < D) {
-            p.o[(it.q_begin + tok) * p.o_ld + static_cast<int64_t>(it.kvh * p.group + h) * D + t] =
-                __float2bfloat16(sum > 0.f ? o / sum : o * 0.f);
+            p.o[(item.x + (at >> 8)) * p.o_ld + static_cast<int64_t>(item.y * p.group + (at & 255)) * D + t] =
+                __float2bfloat16(sum > 0.f ? v / sum : v * 0.f);
           }
         }
       }
-      if (it.n > 0) {
-        tc_fence_before_sync();
-        few_any<256>(3, false);                      // sRed, sM and the row tables have been read
-        if (lane == 0) {
-          mbar_arrive(&o_empty[ob]);
-          mbar_arrive(&t_empty[tb]);
-        }
-      }
-      g0 += it.n;
+      tc_fence_before_sync();
+      few_any<128>(bar, false);                      // sums, maxima and the row tables have been read
+      if (lane == 0) mbar_arrive(&t_empty[tb]);
     }
   }
 

@@ -55,7 +55,8 @@ inline int make_tmap_2d(CUtensorMap* map, CUtensorMapDataType dt, int elem_bytes
 // 3-D tensor [d2, d1, d0(inner)] with byte strides s1 (d1) and s2 (d2).
 inline int make_tmap_3d(CUtensorMap* map, CUtensorMapDataType dt, int elem_bytes, const void* base, uint64_t d0,
                         uint64_t d1, uint64_t d2, uint64_t s1_bytes, uint64_t s2_bytes, uint32_t b0, uint32_t b1,
-                        uint32_t b2, CUtensorMapSwizzle swz = CU_TENSOR_MAP_SWIZZLE_128B) {
+                        uint32_t b2, CUtensorMapSwizzle swz = CU_TENSOR_MAP_SWIZZLE_128B,
+                        CUtensorMapL2promotion fetch = CU_TENSOR_MAP_L2_PROMOTION_L2_256B) {
   EncodeTiledFn fn = get_encode_tiled();
   if (fn == nullptr) return -1;
   if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0 || (s1_bytes & 15u) != 0 || (s2_bytes & 15u) != 0) return -2;
@@ -64,7 +65,7 @@ inline int make_tmap_3d(CUtensorMap* map, CUtensorMapDataType dt, int elem_bytes
   cuuint32_t box[3] = {b0, b1, b2};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = fn(map, dt, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  fetch, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   (void)elem_bytes;
   return r == CUDA_SUCCESS ? 0 : -3;
 }
