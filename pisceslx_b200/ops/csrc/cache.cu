@@ -329,7 +329,7 @@ template <int D>
 int launch_join(const CacheFewParams& f, int rows, int ctas, cudaStream_t stream) {
   auto kernel = rows == 4 ? cache_few_join_kernel<D, 4> : rows == 8 ? cache_few_join_kernel<D, 8> : rows == 16 ? cache_few_join_kernel<D, 16>
                 : rows == 32 ? cache_few_join_kernel<D, 32> : cache_few_join_kernel<D, 64>;
-  return launch_chained(kernel, dim3(f.a.hk, f.a.batch), dim3(128), 0, stream, 0, f, ctas);
+  return launch_chained(kernel, dim3(f.a.hk, f.a.batch, rows / 4), dim3(128), 0, stream, 0, f, ctas);
 }
 
 // One launch over up to kFewSequences sequences; rows of sequences without cu_q begin at first_row.
@@ -344,9 +344,13 @@ int launch_cache_few(const CacheAttnArgs& a, int rows, int first_row, cudaStream
   p.po = static_cast<float*>(a.scratch);
   p.pml = p.po + static_cast<int64_t>(ctas) * 4 * rows * a.d;
   f.pre = reinterpret_cast<int*>(p.pml + static_cast<int64_t>(ctas) * 4 * rows * 2);
-  f.q = static_cast<const __nv_bfloat16*>(a.q); f.q_ld = a.q_ld;
   const bool f8 = a.k_scale != nullptr;
-  int r;
+  p.per_tile = rows / p.group;
+  int r = make_tmap_3d(&f.tma_q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.q, static_cast<uint64_t>(a.d), static_cast<uint64_t>(a.hq),
+                       static_cast<uint64_t>(a.total_q), static_cast<uint64_t>(a.d) * 2, static_cast<uint64_t>(a.q_ld) * 2,
+                       static_cast<uint32_t>(f8 ? a.d : 64), static_cast<uint32_t>(p.group), static_cast<uint32_t>(p.per_tile),
+                       f8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B);
+  if (r != 0) return -10 + r;
   if (f8) {
     if (!al16(a.k_scale) || !al16(a.v_scale)) return -5;
     f.ks = static_cast<const uint8_t*>(a.k_scale); f.vs = static_cast<const uint8_t*>(a.v_scale);

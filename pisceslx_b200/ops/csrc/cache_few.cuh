@@ -25,9 +25,10 @@
 //   10, 11      TMA, a piece each: a stage holds a tile of keys and values (and, of 8-bit pages, their exponent bytes), and what the
 //               other warps have to know of it
 //   12..15      (8-bit pages) values to fp16
-// Only warps 9 to 11 walk the line, and the loops of the others are short: 16 warps in six roles share an instruction cache.  With a
-// walk of both pieces in each of them a third of all stalls was for instructions and an 8-bit tile took 1.5 to 1.8 us; with one
-// warp that copied for both pieces, 1.2.
+// Only warps 9 to 11 walk the line, and all loops are short: 16 warps in six roles share an instruction cache.  With a walk of both
+// pieces in each of them a third of all stalls was for instructions and an 8-bit tile took 1.5 to 1.8 us; with one warp that
+// copied for both pieces, 1.2.  For the same reason 16 rows at a time go through a loop that is not unrolled: with all 64 of a tile
+// unrolled, in registers, what is done once an item cost more than its tiles (18 sequences of 2048 tokens, 16 new ones: 270 us).
 #pragma once
 #include "cache_attn.cuh"
 #include "chain.cuh"
@@ -36,8 +37,7 @@ namespace yv {
 
 struct CacheFewParams {
   CUtensorMap tma_k, tma_v;          // (D, key head, slot): bf16 box (64, 1, box), codes box (D, 1, box)
-  const __nv_bfloat16* q;
-  int64_t q_ld;
+  CUtensorMap tma_q;                 // (D, query head, token): box (64, G, R / G), for 8-bit pages (D, G, R / G) as it lies
   const uint8_t *ks, *vs;
   CacheAttnParams a;                 // po, pml: [piece][2][R][D] and [piece][2][R][2]
   int* pre;                          // [batch + 1] tiles in front of every sequence, for the second kernel
@@ -50,15 +50,14 @@ template <int D, bool F8, int R>
 struct CacheFew {
   static constexpr int kN = R < 16 ? 16 : R;
   static constexpr int kThreads = F8 ? 512 : 384;
-  // registers of the softmax warps and of the others, where 16 rows or more need a split: together what the block was launched with
-  static constexpr int kSoftmaxRegs = F8 ? 168 : 208, kOtherRegs = 88;
   static constexpr int kHalf = kCaTile * D * (F8 ? 1 : 2);           // keys, or values, of a stage
   static constexpr int kStage = 2 * kHalf;                           // values, then keys
   static constexpr int kQ = 2 * kN * D;                              // bf16 rows, or two rows of codes
   static constexpr int kP = kN * kCaTile * 2;
   static constexpr int kWide = F8 ? kCaTile * D * 2 : 0;             // values in fp16
-  static constexpr int kFixed = 2 * (kQ + kP + kWide);               // each of the two pieces has its own
-  static constexpr int kRest = 256 + 4 * (2 * kCaTile + 32) + 22 * kN * 4 + 128 + 13 * kFewSequences + 64;   // barriers, exponent bytes, tables
+  static constexpr int kRaw = F8 ? R * D * 2 : 0;                    // query rows before they become codes
+  static constexpr int kFixed = 2 * (kQ + kP + kWide) + kRaw;        // each of the two pieces has its own
+  static constexpr int kRest = 256 + 4 * (2 * kCaTile + 32) + 30 * kN * 4 + 128 + 13 * kFewSequences + 64;   // barriers, exponent bytes, tables
   static constexpr int kMost = (227 * 1024 - 1024 - kRest - kFixed) / kStage;
   static constexpr int kStages = kMost < 4 ? kMost : 4;
   // 8-bit stages are given back as soon as their keys are multiplied and the rest is read, where a piece's tiles keep to stages of
@@ -71,7 +70,6 @@ struct CacheFew {
   static constexpr uint32_t kCols = kUsed <= 64 ? 64 : kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;
   static_assert(kStages >= 2 && kTotal <= 227 * 1024 && kUsed <= 512, "room");
 };
-static_assert(2 * 168 + 2 * 88 == 4 * 128 && 2 * 208 + 88 == 3 * 168, "register shares");
 
 // Places of the line in front of piece c of n.
 __device__ __forceinline__ int few_cut(int all, int c, int n) { return static_cast<int>(static_cast<int64_t>(all) * c / n); }
@@ -173,6 +171,38 @@ __device__ __forceinline__ int few_place(int row, int place) {
   return BYTES == 128 ? place ^ (row & 7) : BYTES == 64 ? place ^ ((row >> 1) & 3) : place ^ ((row >> 2) & 1);
 }
 
+// v[i] of all lanes joined: a lane's result is that of row lane / (32 / C).  Every step halves the rows that a lane holds.
+template <int C, typename F>
+__device__ __forceinline__ float few_across(const float (&in)[C], int lane, F&& join) {
+  float v[C];
+#pragma unroll
+  for (int i = 0; i < C; ++i) v[i] = in[i];
+#pragma unroll
+  for (int step = 0; step < 5; ++step) {
+    const int bit = 16 >> step, half = C >> (step + 1);
+    const bool up = (lane & bit) != 0;
+    if (half == 0) {
+      v[0] = join(v[0], __shfl_xor_sync(0xFFFFFFFFu, v[0], bit));
+    } else {
+#pragma unroll
+      for (int i = 0; i < half; ++i) {
+        const float other = __shfl_xor_sync(0xFFFFFFFFu, up ? v[i] : v[i + half], bit);
+        v[i] = join(up ? v[i + half] : v[i], other);
+      }
+    }
+  }
+  return v[0];
+}
+
+// four consecutive columns of this thread's TMEM lane
+__device__ __forceinline__ void few_ld4(uint32_t at, uint32_t (&r)[4]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+
+__device__ __forceinline__ void few_st4(uint32_t at, const uint32_t (&r)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
+
 // 8 e4m3 codes -> 8 fp16 numbers, exactly
 __device__ __forceinline__ uint4 few_halves(uint32_t a, uint32_t b) {
   uint4 r;
@@ -228,7 +258,6 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
   constexpr uint32_t kIdescS = F8 ? make_idesc_e4m3(128, 2 * N) : make_idesc_bf16(128, N, false, false);
   // the format fields of fp16 are zero
   constexpr uint32_t kIdescPV = make_idesc_bf16(128, N, true, true) & (F8 ? ~((1u << 7) | (1u << 10)) : ~0u);
-  constexpr bool kShares = R >= 16;
 
   extern __shared__ uint8_t cf_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(cf_raw) + 1023) & ~uintptr_t(1023));
@@ -238,7 +267,8 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
   uint8_t* sRing = sWide + 2 * S::kWide;
   uint8_t* sP = sRing + kStages * S::kStage;                         // [2]
   uint8_t* sQ = sP + 2 * S::kP;                                      // [2]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sQ + 2 * S::kQ);
+  uint8_t* sRaw = sQ + 2 * S::kQ;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sRaw + S::kRaw);
   uint64_t* full = bars;                     // [kStages] keys, values and exponent bytes have landed
   uint64_t* empty = bars + kStages;          // [kStages]
   // of a piece:
@@ -249,7 +279,8 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
   uint64_t* q_empty = v_full + 2;            // [2] query rows
   uint64_t* q_full = q_empty + 2;            // [2][2] query rows and their tables, of which there are two
   uint64_t* t_empty = q_full + 4;            // [2][2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(t_empty + 4);
+  uint64_t* raw_full = t_empty + 4;          // query rows as they were
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(raw_full + 1);
   uint8_t* sByte = reinterpret_cast<uint8_t*>(bars) + 256;                               // [kStages][2][128]
   CacheFewTile* sTile = reinterpret_cast<CacheFewTile*>(sByte + kStages * 2 * kCaTile);  // [kStages]
   volatile int* sFirst = reinterpret_cast<int*>(bars) + 60;                              // [2] whether the weights are an item's first
@@ -258,8 +289,9 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
   int* sRow = sHi + 4 * N;                                                               // [2][2][N] token << 8 | head of the group
   float* sFactor = reinterpret_cast<float*>(sRow + 4 * N);                               // [2][2][N] a row's power of two times the scale
   float* sM = sFactor + 4 * N;                                                           // [2][N] reference maxima
-  float* sRed = sM + 2 * N;                                                              // [2][4][N]; a new maximum goes to [0]
-  int* sTop = reinterpret_cast<int*>(sRed + 8 * N);                                      // [2][8] largest exponent bytes, reference
+  float* sRed = sM + 2 * N;                                                              // [2][4][N] maxima of the warps; a new one goes to [0]
+  float* sSum = sRed + 8 * N;                                                            // [2][4][N] sums of the warps
+  int* sTop = reinterpret_cast<int*>(sSum + 8 * N);                                      // [2][8] largest exponent bytes, reference
   CacheFewTable tab;
   tab.pre = sTop + 16;
   tab.q0 = tab.pre + kFewSequences + 1;
@@ -271,6 +303,7 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
   if (tid == 0) {
     tma_prefetch_desc(&fp.tma_k);
     tma_prefetch_desc(&fp.tma_v);
+    tma_prefetch_desc(&fp.tma_q);
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], S::kEarly ? 9 : 1);         // early: the score product, four softmax warps, four widening ones
@@ -282,8 +315,9 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
       mbar_init(&v_full[i], 4);
       mbar_init(&q_empty[i], 1);
     }
+    mbar_init(raw_full, 1);
     for (int i = 0; i < 4; ++i) {
-      mbar_init(&q_full[i], 1);
+      mbar_init(&q_full[i], F8 ? 1 : 2);     // the tables, and where they are copied as they are the rows
       mbar_init(&t_empty[i], 4);
     }
     fence_barrier_init();
@@ -357,7 +391,6 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
   auto piece_of = [&](uint32_t group) { return static_cast<int>(blockIdx.x + ((group ^ extra) != 0u ? gridDim.x : 0u)); };
   const int both = tiles_of(piece_of(0)) + tiles_of(piece_of(1));
 
-  if (kShares && warp >= 8) regs_give<S::kOtherRegs>();
   if (warp == 10 || warp == 11) {
     // ------------------------------------ copies --------------------------------------------
     const uint32_t grp = warp - 10, lead = elect_one() ? 1u : 0u;
@@ -419,7 +452,8 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
     // ------------------------------------ query rows ----------------------------------------
     // Items of both pieces, in the order in which their first tiles are multiplied.
     const int n0 = tiles_of(piece_of(0));
-    uint32_t items[2] = {0u, 0u}, k[2] = {0u, 0u};                   // items and tiles so far
+    const uint32_t lead = elect_one() ? 1u : 0u;
+    uint32_t items[2] = {0u, 0u}, k[2] = {0u, 0u}, fills = 0;        // items and tiles so far, copies of query rows
     CacheFewItem now, then;
     uint32_t grp = 0;
     now.begin_walk(p, tab, pieces, piece_of(0));
@@ -439,85 +473,76 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
       it.next(p, tab);
       const uint32_t item = grp != 0 ? items[1] : items[0], tb = grp * 2 + (item & 1u);
       if (!few_wait_warp(&q_empty[grp], (item & 1u) ^ 1u, p.status) || !few_wait_warp(&t_empty[tb], ((item >> 1) & 1u) ^ 1u, p.status)) break;
-      if (lane == 0) sItem[tb] = make_int4(it.q_begin, it.kvh, it.slot, 0);
-      constexpr int E = D / 32;                                      // numbers of a lane
-      uint8_t* dst = sQ + grp * S::kQ;
-      constexpr int kAhead = R < 16 ? R : 16;                        // rows whose loads are under way together
-#pragma unroll 1
-      for (int i0 = 0; i0 < R; i0 += kAhead) {
-      uint32_t all[kAhead][E / 2];
-      int tok = i0 / p.group, h = i0 - tok * p.group, row_of[kAhead];
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        const bool there = tok < it.q_len;
-        row_of[i] = there ? tok << 8 | h : -1;
-#pragma unroll
-        for (int e = 0; e < E / 2; ++e) all[i][e] = 0;
-        if (there) {
-          const __nv_bfloat16* src = fp.q + static_cast<int64_t>(it.q_begin + tok) * fp.q_ld + static_cast<int64_t>(it.kvh * p.group + h) * D + lane * E;
-          if constexpr (E == 4) {
-            const uint2 x = *reinterpret_cast<const uint2*>(src);
-            all[i][0] = x.x;
-            all[i][1] = x.y;
-          } else {
-            all[i][0] = *reinterpret_cast<const uint32_t*>(src);
-          }
+      const int box = p.group * p.per_tile;                          // rows of the copy
+      if constexpr (F8) {
+        if (lead) {
+          mbar_expect_tx(raw_full, static_cast<uint32_t>(box) * D * 2);
+          tma_load_3d(sRaw, &fp.tma_q, raw_full, 0, it.kvh * p.group, it.q_begin);
         }
-        if (++h == p.group) {
-          h = 0;
-          ++tok;
-        }
+      } else if (lead) {
+        mbar_expect_tx(&q_full[tb], static_cast<uint32_t>(box) * D * 2);
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+          tma_load_3d(sQ + grp * S::kQ + c * (N * 128), &fp.tma_q, &q_full[tb], c * 64, it.kvh * p.group, it.q_begin);
       }
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const int i = i0 + k;
-        const uint32_t* w = all[k];
-        float factor = p.scale_log2;
-        if constexpr (F8) {
-          uint32_t top = 0;
-#pragma unroll
-          for (int e = 0; e < E / 2; ++e) top = max(top, max(w[e] & 0x7FFFu, (w[e] >> 16) & 0x7FFFu));
-          top = __reduce_max_sync(0xFFFFFFFFu, top);
-          const bool finite = top < 0x7F80u;
-          const int byte = finite ? max(0, static_cast<int>(top >> 7) - 8 + ((top & 0x7Fu) > 0x60u ? 1 : 0)) : 127;
-          const float inv = __int_as_float((254 - byte) << 23);      // 2^-E
-          factor = finite ? factor * (byte == 0 ? __int_as_float(0x00400000) : __int_as_float(byte << 23)) : __int_as_float(0x7FC00000);
-          uint32_t c1 = 0, c2 = 0;
-#pragma unroll
-          for (int e = 0; e < E / 2; ++e) {
-            const float2 x = make_float2(__uint_as_float(w[e] << 16) * inv, __uint_as_float(w[e] & 0xFFFF0000u) * inv);
-            const __nv_fp8x2_storage_t a = __nv_cvt_float2_to_fp8x2(x, __NV_SATFINITE, __NV_E4M3);
-            const float2 y = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(a, __NV_E4M3)));
-            const __nv_fp8x2_storage_t b =
-                __nv_cvt_float2_to_fp8x2(make_float2((x.x - y.x) * 16.f, (x.y - y.y) * 16.f), __NV_SATFINITE, __NV_E4M3);
-            c1 |= static_cast<uint32_t>(a) << (16 * e);
-            c2 |= static_cast<uint32_t>(b) << (16 * e);
-          }
-          if (!finite) c1 = c2 = 0;
-          // rows i and N + i (N is a multiple of 16: the same exchange of places)
-          const uint32_t at = (few_place<D>(i, (lane * E) >> 4) << 4) + ((lane * E) & 15);
-          if constexpr (D == 128) {
-            *reinterpret_cast<uint32_t*>(dst + i * D + at) = c1;
-            *reinterpret_cast<uint32_t*>(dst + (N + i) * D + at) = c2;
-          } else {
-            *reinterpret_cast<uint16_t*>(dst + i * D + at) = static_cast<uint16_t>(c1);
-            *reinterpret_cast<uint16_t*>(dst + (N + i) * D + at) = static_cast<uint16_t>(c2);
-          }
-        } else if constexpr (E == 4) {
-          const int c = lane >> 1;
-          *reinterpret_cast<uint2*>(dst + (c >> 3) * (N * 128) + i * 128 + (few_place<128>(i, c & 7) << 4) + ((lane & 1) << 3)) = make_uint2(w[0], w[1]);
-        } else {
-          *reinterpret_cast<uint32_t*>(dst + i * 128 + (few_place<128>(i, lane >> 2) << 4) + ((lane & 3) << 2)) = w[0];
-        }
-        if (lane == 0) {
-          sHi[tb * N + i] = row_of[k] >= 0 ? (row_of[k] >> 8) + it.shift : -1;
-          sRow[tb * N + i] = row_of[k];
-          sFactor[tb * N + i] = factor;
-        }
-      }
-      }
-      fence_proxy_async_smem();
       __syncwarp();
+      if (lane == 0) sItem[tb] = make_int4(it.q_begin, it.kvh, it.slot, 0);
+      for (int i = lane; i < R; i += 32) {
+        const int tok = i / p.group;
+        sHi[tb * N + i] = tok < it.q_len ? tok + it.shift : -1;
+        sRow[tb * N + i] = tok < it.q_len ? tok << 8 | (i - tok * p.group) : -1;
+      }
+      if constexpr (F8) {
+        // Four lanes for a row, eight rows at a time: the row's power of two, and two codes for each number.
+        if (!few_wait_warp(raw_full, fills & 1u, p.status)) break;
+        ++fills;
+        uint8_t* dst = sQ + grp * S::kQ;
+        const int part = lane & 3;
+#pragma unroll 1
+        for (int i = lane >> 2; i < (R < 8 ? 8 : R); i += 8) {
+          const bool there = i / p.group < it.q_len && i < R;
+          constexpr int kVecs = D / 32;                              // 16-byte vectors of a lane
+          uint4 x[kVecs];
+          uint32_t m2 = 0;
+#pragma unroll
+          for (int v = 0; v < kVecs; ++v) {
+            x[v] = there ? *reinterpret_cast<const uint4*>(sRaw + i * D * 2 + (part * kVecs + v) * 16) : make_uint4(0, 0, 0, 0);
+            m2 = __vmaxu2(__vmaxu2(m2, x[v].x & 0x7FFF7FFFu), __vmaxu2(x[v].y & 0x7FFF7FFFu, __vmaxu2(x[v].z & 0x7FFF7FFFu, x[v].w & 0x7FFF7FFFu)));
+          }
+          uint32_t most = max(m2 & 0xFFFFu, m2 >> 16);
+          most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
+          most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
+          const bool finite = most < 0x7F80u;
+          const int byte = finite ? max(0, static_cast<int>(most >> 7) - 8 + ((most & 0x7Fu) > 0x60u ? 1 : 0)) : 127;
+          const float inv = __int_as_float((254 - byte) << 23);      // 2^-E
+#pragma unroll
+          for (int v = 0; v < kVecs; v += 2) {
+            const uint32_t w[8] = {x[v].x, x[v].y, x[v].z, x[v].w, x[v + 1].x, x[v + 1].y, x[v + 1].z, x[v + 1].w};
+            uint32_t c1[4] = {0, 0, 0, 0}, c2[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float2 f = make_float2(__uint_as_float(w[e] << 16) * inv, __uint_as_float(w[e] & 0xFFFF0000u) * inv);
+              const __nv_fp8x2_storage_t a = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
+              const float2 y = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(a, __NV_E4M3)));
+              const __nv_fp8x2_storage_t b =
+                  __nv_cvt_float2_to_fp8x2(make_float2((f.x - y.x) * 16.f, (f.y - y.y) * 16.f), __NV_SATFINITE, __NV_E4M3);
+              c1[e / 2] |= static_cast<uint32_t>(a) << (16 * (e & 1));
+              c2[e / 2] |= static_cast<uint32_t>(b) << (16 * (e & 1));
+            }
+            // rows i and N + i (N is a multiple of 16: the same exchange of places)
+            const int at = few_place<D>(i, (part * kVecs + v) / 2) << 4;
+            if (i < R) {
+              *reinterpret_cast<uint4*>(dst + i * D + at) = finite ? make_uint4(c1[0], c1[1], c1[2], c1[3]) : make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(dst + (N + i) * D + at) = finite ? make_uint4(c2[0], c2[1], c2[2], c2[3]) : make_uint4(0, 0, 0, 0);
+            }
+          }
+          if (part == 0 && i < R)
+            sFactor[tb * N + i] = finite ? p.scale_log2 * few_power(byte) : __int_as_float(0x7FC00000);
+        }
+        fence_proxy_async_smem();
+      }
+      __syncwarp();
+      // (of bf16 pages the copy's arrival is announced above: this one is the tables')
       if (lane == 0) mbar_arrive(&q_full[tb]);
       if (grp != 0) { ++items[1]; k[1] += it.n; } else { ++items[0]; k[0] += it.n; }
     }
@@ -626,7 +651,6 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
     }
   } else if (warp < 8) {
     // ------------------------------------ softmax -------------------------------------------
-    if constexpr (kShares) regs_take<S::kSoftmaxRegs>();
     const uint32_t grp = warp >> 2;                                  // the piece of this warp
     const int t = tid & 127, bar = 1 + grp;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -638,148 +662,148 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
     bool ok = true;
     const int piece = piece_of(grp);
     const uint32_t mine = tiles_of(piece), others = both - mine;
-    float l[R];
+    constexpr int C = R < 16 ? R : 16;                               // rows at a time
+    float* sums = sSum + (grp * 4 + (warp & 3)) * N;
+    const int my_row = lane / (32 / C);                              // whose joined value this lane holds
+    const bool my_turn = lane % (32 / C) == 0;
     for (; k < mine; ++k) {
       const uint32_t g = few_turn(k, grp, others), s = g % kStages, ph = k & 1u;
       const uint32_t tb = grp * 2 + (items & 1u);
       // a warp whose wait ran out (what it reads of the tile may then be anything) goes to the vote; the group leaves there together
       ok = ok && few_wait(&full[s], (g / kStages) & 1u, p.status);
       const int flags = sTile[s].flags, key = sTile[s].key + t;
-      const bool first = (flags & kFewFirst) != 0;                   // the group's maxima and reference are an earlier item's
-      if (first) {
+      const bool first = (flags & kFewFirst) != 0;                   // the group's maxima, sums and reference are an earlier item's
+      const bool seen = (flags & kFewWhole) != 0 || sTile[s].seen(key);
+      if (first) ok = ok && few_wait(&q_full[tb], (items >> 1) & 1u, p.status);
+      ok = ok && few_wait(&s_full[grp], ph, p.status);
+      ok = __all_sync(0xFFFFFFFFu, ok);                              // the aligned tcgen05 instructions need a converged warp
+      float kf = p.scale_log2;
+      int vbyte = 0;
+      bool high = first;
+      float sc[C];
+      // scores of C rows from n0 on (log2 domain)
+      auto scores = [&](int n0) {
+        uint32_t a[16];
+        tmem_ld16(tS + n0, a);
+        if constexpr (F8) {
+          uint32_t b[16];
+          tmem_ld16(tS + N + n0, b);
+          float f[C];
 #pragma unroll
-        for (int i = 0; i < R; ++i) l[i] = 0.f;
-        ok = ok && few_wait(&q_full[tb], (items >> 1) & 1u, p.status);
-      }
-      {
-        const bool seen = (flags & kFewWhole) != 0 || sTile[s].seen(key);
-        ok = ok && few_wait(&s_full[grp], ph, p.status);
-        ok = __all_sync(0xFFFFFFFFu, ok);                            // the aligned tcgen05 instructions need a converged warp
-        float sc[R];
-        bool high = first;
-        int vbyte = 0;
-        if (ok) {
-          tc_fence_after_sync();
-          float kf = p.scale_log2;
-          if (F8) {
-            kf = few_power(sByte[s * 2 * kCaTile + t]);
-            vbyte = seen ? sByte[s * 2 * kCaTile + kCaTile + t] : 0;
-            __syncwarp();
-            if (S::kEarly && lane == 0) mbar_arrive(&empty[s]);
-            high |= vbyte > top[7] + 3 && vbyte != 255;              // NaN needs no reference
+          for (int i = 0; i < C; i += 4) *reinterpret_cast<float4*>(f + i) = *reinterpret_cast<const float4*>(sFactor + tb * N + n0 + i);
+          tc_wait_ld();
+#pragma unroll
+          for (int i = 0; i < C; ++i) sc[i] = fmaf(__uint_as_float(b[i]), 0.0625f, __uint_as_float(a[i])) * (kf * f[i]);
+        } else {
+          tc_wait_ld();
+#pragma unroll
+          for (int i = 0; i < C; ++i) sc[i] = __uint_as_float(a[i]) * kf;
+        }
+        if ((flags & kFewAll) == 0) {
+#pragma unroll
+          for (int i = 0; i < C; ++i) {
+            const int hi = sHi[tb * N + n0 + i];
+            if (!(seen && key <= hi && (p.window == 0 || key > hi - p.window || key < p.first))) sc[i] = kCaMask;
           }
+        }
+      };
+      if (ok) {
+        tc_fence_after_sync();
+        if constexpr (F8) {
+          kf = few_power(sByte[s * 2 * kCaTile + t]);
+          vbyte = seen ? sByte[s * 2 * kCaTile + kCaTile + t] : 0;
+          __syncwarp();
+          if (S::kEarly && lane == 0) mbar_arrive(&empty[s]);
+          high |= vbyte > top[7] + 3 && vbyte != 255;                // NaN needs no reference
+        }
+#pragma unroll 1
+        for (int n0 = 0; n0 < R; n0 += C) {
+          scores(n0);
 #pragma unroll
-          for (int n0 = 0; n0 < N; n0 += 16) {
-            constexpr int kHere = R < 16 ? R : 16;
-            uint32_t a[16];
-            tmem_ld16(tS + n0, a);
-            if constexpr (F8) {
-              uint32_t b[16];
-              tmem_ld16(tS + N + n0, b);
-              float f[kHere];
-#pragma unroll
-              for (int i = 0; i < kHere; i += 4) *reinterpret_cast<float4*>(f + i) = *reinterpret_cast<const float4*>(sFactor + tb * N + n0 + i);
-              tc_wait_ld();
-#pragma unroll
-              for (int i = 0; i < kHere; ++i)
-                sc[n0 + i] = fmaf(__uint_as_float(b[i]), 0.0625f, __uint_as_float(a[i])) * (kf * f[i]);
-            } else {
-              tc_wait_ld();
-#pragma unroll
-              for (int i = 0; i < kHere; ++i) sc[n0 + i] = __uint_as_float(a[i]) * kf;
-            }
-          }
-          if ((flags & kFewAll) == 0) {
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-              const int hi = sHi[tb * N + i];
-              if (!(seen && key <= hi && (p.window == 0 || key > hi - p.window || key < p.first))) sc[i] = kCaMask;
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < R; i += 4) {
-            const float4 m = *reinterpret_cast<const float4*>(m_mine + i);
+          for (int i = 0; i < C; i += 4) {
+            const float4 m = *reinterpret_cast<const float4*>(m_mine + n0 + i);
             high |= !(sc[i] <= m.x + kCaRescale) || !(sc[i + 1] <= m.y + kCaRescale) || !(sc[i + 2] <= m.z + kCaRescale) ||
                     !(sc[i + 3] <= m.w + kCaRescale);
           }
         }
-        tc_fence_before_sync();
-        // lazy: a reference maximum moves only when a score exceeds it by more than 2^8 (or is NaN)
-        const bool moves = few_any<128>(bar, high || !ok);
-        // the product of the group's last tile has landed: its P buffer is free, its sums may be rescaled
-        if (k > 0) ok = ok && few_wait(&pv_done[grp], ph ^ 1u, p.status);
-        ok = __all_sync(0xFFFFFFFFu, ok);
-        if (moves) {
-          if (ok) {
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-              float v = sc[i];
-#pragma unroll
-              for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
-              if (lane == 0) red[(warp & 3) * N + i] = v;
-            }
-            if (F8) {
-              const int v = __reduce_max_sync(0xFFFFFFFFu, vbyte == 255 ? 0 : vbyte);
-              if (lane == 0) top[warp & 3] = v;
-            }
-          }
-          ok = !few_any<128>(bar, !ok);
-          if (!ok) break;
-          // a reference exponent that is passed by more than 3 moves as the maxima do
-          const int old_ref = !F8 ? 0 : first ? -1024 : top[7], most = F8 ? max(max(top[0], top[1]), max(top[2], top[3])) : 0;
-          const int ref = most > old_ref + 3 ? most : old_ref;
-          const float rescale = F8 ? ex2(static_cast<float>(old_ref - ref)) : 1.f;
-          if (t < R) {
-            const float now = max_nan(max_nan(red[t], red[N + t]), max_nan(red[2 * N + t], red[3 * N + t]));
-            const float old = first ? -1.0e29f : m_mine[t];
-            red[t] = !(now <= old + kCaRescale) ? now : old;
-          }
-          few_any<128>(bar, false);
+      }
+      tc_fence_before_sync();
+      // lazy: a reference maximum moves only when a score exceeds it by more than 2^8 (or is NaN)
+      const bool moves = few_any<128>(bar, high || !ok);
+      // the product of the group's last tile has landed: its P buffer is free, its sums may be rescaled
+      if (k > 0) ok = ok && few_wait(&pv_done[grp], ph ^ 1u, p.status);
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (moves) {
+        if (ok) {
           tc_fence_after_sync();
+#pragma unroll 1
+          for (int n0 = 0; n0 < R; n0 += C) {
+            if (R > C) scores(n0);
+            const float v = few_across<C>(sc, lane, [](float x, float y) { return max_nan(x, y); });
+            if (my_turn) red[(warp & 3) * N + n0 + my_row] = v;
+          }
+          if (F8) {
+            const int v = __reduce_max_sync(0xFFFFFFFFu, vbyte == 255 ? 0 : vbyte);
+            if (lane == 0) top[warp & 3] = v;
+          }
+        }
+        ok = !few_any<128>(bar, !ok);
+        if (!ok) break;
+        // a reference exponent that is passed by more than 3 moves as the maxima do
+        const int old_ref = !F8 ? 0 : first ? -1024 : top[7], most = F8 ? max(max(top[0], top[1]), max(top[2], top[3])) : 0;
+        const int ref = most > old_ref + 3 ? most : old_ref;
+        const float rescale = F8 ? ex2(static_cast<float>(old_ref - ref)) : 1.f;
+        if (t < R) {
+          const float now = max_nan(max_nan(red[t], red[N + t]), max_nan(red[2 * N + t], red[3 * N + t]));
+          const float old = first ? -1.0e29f : m_mine[t];
+          red[t] = !(now <= old + kCaRescale) ? now : old;
+        }
+        few_any<128>(bar, false);
+        if (!first) {
+          tc_fence_after_sync();
+#pragma unroll 1
+          for (int n0 = 0; n0 < R; n0 += 4) {
+            uint32_t o[4];
+            few_ld4(to + n0, o);
+            tc_wait_ld();
 #pragma unroll
-          for (int n0 = 0; n0 < N; n0 += 16) {
-            constexpr int kHere = R < 16 ? R : 16;
-            uint32_t o[16];
-            if (!first) {
-              tmem_ld16(to + n0, o);
-              tc_wait_ld();
-            }
-#pragma unroll
-            for (int i = 0; i < kHere; ++i) {
-              const float alpha = first ? 1.f : ex2(m_mine[n0 + i] - red[n0 + i]);
-              l[n0 + i] *= alpha;
-              if (!first) o[i] = __float_as_uint(__uint_as_float(o[i]) * (F8 ? alpha * rescale : alpha));
-            }
-            if (!first) {
-              tmem_st16(to + n0, o);
-              tc_wait_st();
-            }
+            for (int i = 0; i < 4; ++i)
+              o[i] = __float_as_uint(__uint_as_float(o[i]) * (ex2(m_mine[n0 + i] - red[n0 + i]) * rescale));
+            few_st4(to + n0, o);
+            tc_wait_st();
           }
           tc_fence_before_sync();
-          few_any<128>(bar, false);                                  // everyone has read the old maxima
-          if (t < R) m_mine[t] = red[t];
-          if (F8 && t == 0) top[7] = ref;
-          few_any<128>(bar, false);
+          if (my_turn)
+            for (int n0 = my_row; n0 < R; n0 += C) sums[n0] *= ex2(m_mine[n0] - red[n0]);
         }
-        if (ok) {
-          // A key's weights are a row of P.  The sums take bf16 weights as rounded, as the tensor core multiplies them; fp16 ones, which
-          // hold the value's exponent as well, before they are rounded.
-          uint32_t w[R / 2];
-          const float vf = vbyte == 255 ? __int_as_float(0x7FC00000) : ex2(static_cast<float>(vbyte - top[7] + 4));
+        few_any<128>(bar, false);                                    // everyone has read the old maxima
+        if (t < R) m_mine[t] = red[t];
+        if (F8 && t == 0) top[7] = ref;
+        few_any<128>(bar, false);
+      }
+      if (ok) {
+        tc_fence_after_sync();
+        // A key's weights are a row of P.  The sums take bf16 weights as rounded, as the tensor core multiplies them; fp16 ones, which
+        // hold the value's exponent as well, before they are rounded.
+        const float vf = vbyte == 255 ? __int_as_float(0x7FC00000) : ex2(static_cast<float>(vbyte - top[7] + 4));
+#pragma unroll 1
+        for (int n0 = 0; n0 < R; n0 += C) {
+          if (R > C) scores(n0);
+          uint32_t w[C / 2];
 #pragma unroll
-          for (int i = 0; i < R; i += 4) {
-            const float4 m = *reinterpret_cast<const float4*>(m_mine + i);
+          for (int i = 0; i < C; i += 4) {
+            const float4 m = *reinterpret_cast<const float4*>(m_mine + n0 + i);
             const float e[4] = {ex2(sc[i] - m.x), ex2(sc[i + 1] - m.y), ex2(sc[i + 2] - m.z), ex2(sc[i + 3] - m.w)};     // masked: 0
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               if constexpr (F8) {
                 w[i / 2 + h] = few_pack_half(e[2 * h] * vf, e[2 * h + 1] * vf);
-                l[i + 2 * h] += e[2 * h];
-                l[i + 2 * h + 1] += e[2 * h + 1];
+                sc[i + 2 * h] = e[2 * h];
+                sc[i + 2 * h + 1] = e[2 * h + 1];
               } else {
                 w[i / 2 + h] = pack_bf16(e[2 * h], e[2 * h + 1]);
-                l[i + 2 * h] += __uint_as_float(w[i / 2 + h] << 16);
-                l[i + 2 * h + 1] += __uint_as_float(w[i / 2 + h] & 0xFFFF0000u);
+                sc[i + 2 * h] = __uint_as_float(w[i / 2 + h] << 16);
+                sc[i + 2 * h + 1] = __uint_as_float(w[i / 2 + h] & 0xFFFF0000u);
               }
             }
           }
@@ -787,51 +811,46 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
             *reinterpret_cast<uint2*>(sp + (few_place<kPRow>(t, 0) << 4)) = make_uint2(w[0], w[1]);
           } else {
 #pragma unroll
-            for (int i = 0; i < R / 8; ++i)
-              *reinterpret_cast<uint4*>(sp + (few_place<kPRow>(t, i) << 4)) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+            for (int i = 0; i < C / 8; ++i)
+              *reinterpret_cast<uint4*>(sp + (few_place<kPRow>(t, n0 / 8 + i) << 4)) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
           }
-          if (!F8 && !seen) {              // values that no row sees are cleared (0 * NaN would be NaN)
+          const float v = few_across<C>(sc, lane, [](float x, float y) { return x + y; });
+          if (my_turn) sums[n0 + my_row] = first ? v : sums[n0 + my_row] + v;
+        }
+        if (!F8 && !seen) {                          // values that no row sees are cleared (0 * NaN would be NaN)
 #pragma unroll
-            for (int c = 0; c < D / 64; ++c)
+          for (int c = 0; c < D / 64; ++c)
 #pragma unroll
-              for (int i = 0; i < 8; ++i) reinterpret_cast<uint4*>(stage_v(s) + c * kSlab + t * 128)[i] = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-          tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) {
-            if ((warp & 3) == 0) sFirst[grp] = first ? 1 : 0;
-            mbar_arrive(&p_full[grp]);
-          }
+            for (int i = 0; i < 8; ++i) reinterpret_cast<uint4*>(stage_v(s) + c * kSlab + t * 128)[i] = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          if ((warp & 3) == 0) sFirst[grp] = first ? 1 : 0;
+          mbar_arrive(&p_full[grp]);
         }
       }
       if ((flags & kFewLast) == 0) continue;
       // ---- the end of an item
       ok = ok && few_wait(&pv_done[grp], ph, p.status);
-#pragma unroll
-      for (int i = 0; i < R; ++i) {
-        float v = l[i];
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-        if (lane == 0) red[(warp & 3) * N + i] = v;
-      }
-      ok = !few_any<128>(bar, !ok);
+      ok = !few_any<128>(bar, !ok);                  // all sums are there
       if (!ok) break;                                // a wait ran out (the status word says so): the outputs are not written
       tc_fence_after_sync();
       const int4 item = sItem[tb];                   // first row of q, key head, slot
       ++items;
       const float back = F8 ? few_power(max(top[7], 0)) * 0.0625f : 1.f;                 // 2^(Eref - 4)
+      const float* all = sSum + grp * 4 * N;
 #pragma unroll 1
-      for (int n0 = 0; n0 < R; n0 += 16) {
-        constexpr int kHere = R < 16 ? R : 16;
-        uint32_t o[16];
-        tmem_ld16(to + n0, o);
+      for (int n0 = 0; n0 < R; n0 += 4) {
+        uint32_t o[4];
+        few_ld4(to + n0, o);
         tc_wait_ld();
 #pragma unroll
-        for (int i = 0; i < kHere; ++i) {
+        for (int i = 0; i < 4; ++i) {
           const int row = n0 + i, at = sRow[tb * N + row];
           if (at < 0) continue;
-          const float sum = (red[row] + red[N + row]) + (red[2 * N + row] + red[3 * N + row]), v = __uint_as_float(o[i]) * back;
+          const float sum = (all[row] + all[N + row]) + (all[2 * N + row] + all[3 * N + row]), v = __uint_as_float(o[i]) * back;
           if (item.z >= 0) {
             const int64_t part = (static_cast<int64_t>(piece) * 2 + item.z) * R + row;
             if (t < D) p.po[part * D + t] = v;
@@ -856,13 +875,13 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
   }
 }
 
-// Joins the parts of a (sequence, head) that was cut: a block for each, most of which leave at once.
+// Joins the parts of a (sequence, head) that was cut: a warp for a row; most blocks leave at once.
 template <int D, int R>
 __global__ void __launch_bounds__(128) cache_few_join_kernel(const CacheFewParams fp, int ctas) {
   const CacheAttnParams& p = fp.a;
   chain_next();
   chain_wait();
-  const int b = blockIdx.y, kvh = blockIdx.x;
+  const int b = blockIdx.y, kvh = blockIdx.x, row = blockIdx.z * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int all = fp.pre[p.batch] * p.hk, pieces = few_pieces(all, ctas);
   const int tiles = fp.pre[b + 1] - fp.pre[b], from = fp.pre[b] * p.hk + kvh * tiles;
   if (tiles == 0) return;
@@ -875,29 +894,37 @@ __global__ void __launch_bounds__(128) cache_few_join_kernel(const CacheFewParam
   };
   const int c0 = piece(from), c1 = piece(from + tiles - 1);
   if (c0 == c1) return;
-  const int first_slot = few_cut(all, c0, pieces) == from ? 0 : 1;
   int q_begin, q_len, k_len;
   ca_sequence(p, b, q_begin, q_len, k_len, false);
-  constexpr int kGroups = 128 / (D / 4);                             // rows at a time, four numbers a thread
-  const int d4 = threadIdx.x % (D / 4);
-  for (int row = threadIdx.x / (D / 4); row < q_len * p.group; row += kGroups) {
-    float m = -1.0e29f, l = 0.f;
-    for (int c = c0; c <= c1; ++c) m = max_nan(m, p.pml[((c * 2 + (c == c0 ? first_slot : 0)) * R + row) * 2]);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int c = c0; c <= c1; ++c) {
-      const int64_t part = (c * 2 + (c == c0 ? first_slot : 0)) * R + row;
-      const float2 ml = *reinterpret_cast<const float2*>(p.pml + part * 2);
-      const float f = ex2(ml.x - m);
-      const float4 o = *reinterpret_cast<const float4*>(p.po + part * D + d4 * 4);
-      l += ml.y * f;
-      acc.x += o.x * f; acc.y += o.y * f; acc.z += o.z * f; acc.w += o.w * f;
+  if (row >= q_len * p.group) return;
+  const int first_slot = few_cut(all, c0, pieces) == from ? 0 : 1;
+  auto part = [&](int c) { return (c * 2 + (c == c0 ? first_slot : 0)) * R + row; };
+  float m = -1.0e29f;
+  for (int c = c0 + lane; c <= c1; c += 32) m = max_nan(m, p.pml[part(c) * 2]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+  constexpr int E = D / 32;
+  float acc[E], l = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll 8
+  for (int c = c0; c <= c1; ++c) {
+    const float2 ml = *reinterpret_cast<const float2*>(p.pml + part(c) * 2);
+    const float f = ex2(ml.x - m);
+    const float* o = p.po + static_cast<int64_t>(part(c)) * D + lane * E;
+    l += ml.y * f;
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      const float2 v = *reinterpret_cast<const float2*>(o + e);
+      acc[e] += v.x * f;
+      acc[e + 1] += v.y * f;
     }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    const int tok = row / p.group, h = row - tok * p.group;
-    *reinterpret_cast<uint2*>(p.o + (q_begin + tok) * p.o_ld + static_cast<int64_t>(kvh * p.group + h) * D + d4 * 4) =
-        make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
   }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const int tok = row / p.group, h = row - tok * p.group;
+  uint32_t* dst = reinterpret_cast<uint32_t*>(p.o + (q_begin + tok) * p.o_ld + static_cast<int64_t>(kvh * p.group + h) * D + lane * E);
+#pragma unroll
+  for (int e = 0; e < E; e += 2) dst[e / 2] = pack_bf16(acc[e] * inv, acc[e + 1] * inv);
 }
 
 }  // namespace yv
