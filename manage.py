@@ -71,6 +71,10 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--host", default="127.0.0.1")
     p.add_argument("--port", type=int, default=8000)
     p.add_argument("--kv_blocks", type=int, default=1024)
+    p.add_argument("--kv_cache_dtype", default="model", choices=["model", "fp8_e4m3"], help="8-bit keys and values in the cache")
+    p.add_argument("--attention_window", type=int, default=None, help="tokens attend to the last N tokens only ...")
+    p.add_argument("--first_tokens", type=int, default=0, help="... and to the first ones of their sequence")
+    p.add_argument("--prefill_portion", type=int, default=0, help="run prompts in portions of at most N tokens")
     # test / benchmark
     p.add_argument("--quick", action="store_true")
     p.add_argument("--gpu", action="store_true")

@@ -29,6 +29,7 @@ import torch
 import torch.nn as nn
 
 from ..config import YvConfig
+from ..ops import cache as C
 from ..ops import functional as F_
 from .norms import YvRMSNorm, YvRotaryEmbedding
 
@@ -205,6 +206,8 @@ class YvAttention(nn.Module):
         nq, nk = self.hq * self.d, self.hk * self.d
         if ctx.cp_group is not None:
             return self._attend_context_parallel(qkv, ctx)
+        if ctx.cache is not None and ctx.slot_map is not None and (any(ctx.starts or ()) or getattr(ctx.cache, "pages_only", False)):
+            return self._attend_pages(qkv, ctx)
         o = F_.rope_attention(qkv, ctx.cos, ctx.sin, ctx.positions, ctx.cu_seqlens, ctx.max_len, self.hq, self.hk,
                               self.d, self.rot_dim, ctx.causal, self.scale, self.deterministic)
         if ctx.cache is not None and ctx.slot_map is not None:
@@ -216,6 +219,51 @@ class YvAttention(nn.Module):
                                        self.rot_dim).reshape(-1, nk)
             F_.kv_cache_write(k_rot.detach(), v_new.detach(), kc, vc, ctx.slot_map)
         return o
+
+    def _rotate(self, qkv: torch.Tensor, ctx: AttnContext) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """Queries and keys of the packed projection, rotated (on the GPU in place), and values."""
+        nq, nk = self.hq * self.d, self.hk * self.d
+        q, k, v = qkv[:, :nq], qkv[:, nq:nq + nk], qkv[:, nq + nk:]
+        if ctx.cos is None:
+            return q, k, v
+        if qkv.is_cuda:
+            F_.rope_(q, k, ctx.cos, ctx.sin, ctx.positions, self.hq, self.hk, self.d, self.rot_dim)
+            return q, k, v
+        from ..ops import reference as ref
+        T = qkv.shape[0]
+        turn = lambda x, h: ref.apply_rope(x.reshape(T, h, self.d), ctx.cos, ctx.sin, ctx.positions, self.rot_dim).reshape(T, h * self.d)
+        return turn(q, self.hq), turn(k, self.hk), v
+
+    def _store(self, k: torch.Tensor, v: torch.Tensor, ctx: AttnContext) -> None:
+        """Rotated keys, and values, into the step's slots of the cache, in the form in which it holds them."""
+        kc, vc = ctx.cache.layer(self.layer_idx)
+        ks, vs = ctx.cache.scales(self.layer_idx)
+        if ks is not None:
+            C.kv_cache_write_fp8(k.detach(), v.detach(), kc, vc, ks, vs, ctx.slot_map)
+        else:
+            F_.kv_cache_write(k.detach(), v.detach(), kc, vc, ctx.slot_map)
+
+    def _attend_pages(self, qkv: torch.Tensor, ctx: AttnContext) -> torch.Tensor:
+        """Attention of a prompt, or of a portion that continues one, over the cache.  A prompt from its start, without a window,
+        meets its own keys and values as they were computed; all else meets what the pages hold."""
+        T, cc = qkv.shape[0], ctx.cache.cfg
+        if cc.attention_window is None and not any(ctx.starts or ()):
+            nq, nk = self.hq * self.d, self.hk * self.d
+            o = F_.rope_attention(qkv, ctx.cos, ctx.sin, ctx.positions, ctx.cu_seqlens, ctx.max_len, self.hq, self.hk, self.d,
+                                  self.rot_dim, ctx.causal, self.scale, self.deterministic)
+            k = qkv[:, nq:nq + nk]
+            if not qkv.is_cuda:
+                k = self._rotate(qkv, ctx)[1]                                  # there the projection is not rotated in place
+            self._store(k, qkv[:, nq + nk:], ctx)
+            return o
+        q, k, v = self._rotate(qkv, ctx)
+        self._store(k, v, ctx)
+        kc, vc = ctx.cache.layer(self.layer_idx)
+        ks, vs = ctx.cache.scales(self.layer_idx)
+        table, lens = ctx.pages()
+        o = C.cache_attention(q.reshape(T, self.hq, self.d) if not q.is_cuda else q.view(T, self.hq, self.d), kc, vc, table, lens,
+                              ctx.cu_seqlens, ctx.max_len, self.scale, cc.attention_window, cc.first_tokens, ks, vs)
+        return o.reshape(T, self.hq * self.d)
 
     def _attend_context_parallel(self, qkv: torch.Tensor, ctx: AttnContext) -> torch.Tensor:
         """Training attention when every sequence is split over the ranks of ``ctx.cp_group`` (contiguous chunks):
@@ -250,6 +298,13 @@ class YvAttention(nn.Module):
         nq, nk = self.hq * self.d, self.hk * self.d
         q, k, v = qkv[:, :nq], qkv[:, nq:nq + nk], qkv[:, nq + nk:]
         kc, vc = ctx.cache.layer(self.layer_idx)
+        if getattr(ctx.cache, "pages_only", False):
+            q, k, v = self._rotate(qkv, ctx)
+            self._store(k, v, ctx)
+            cc = ctx.cache.cfg
+            o = C.cache_attention(q.view(B, self.hq, self.d), kc, vc, ctx.block_table, ctx.seq_lens, None, 1, self.scale,
+                                  cc.attention_window, cc.first_tokens, *ctx.cache.scales(self.layer_idx))
+            return o.reshape(B, nq)
         if ctx.cos is not None and qkv.is_cuda:
             F_.rope_cache(q, k, v, ctx.cos, ctx.sin, ctx.positions, self.hq, self.hk, self.d, self.rot_dim, kc, vc, ctx.slot_map)
         else:

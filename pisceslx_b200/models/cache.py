@@ -7,7 +7,10 @@ quantisation, eviction; cache.py:1886-2038).  Here the cache is two device tenso
 reads pages in place.  ``YvPagedLayeredCache`` keeps the same pages, tables and free list for layer runs that each store
 what they need (keys and values of sizes of their own, or one latent row per token), and gives pages back once every
 layer's window has passed them.  The cache is exact; eviction policies (LRU of whole sequences, sliding window) are
-opt-in helpers that only edit block tables.
+opt-in helpers that only edit block tables.  Two more options are opt-in and lossy.  With ``dtype`` float8_e4m3fn ``YvPagedKVCache`` holds
+keys and values as 8-bit codes and one exponent byte for each token and head (``ops.cache``), a little over half the bytes of
+bf16.  With ``attention_window`` a token attends to the last ``attention_window`` tokens and to the ``first_tokens`` first of its
+sequence (streaming attention: the first tokens carry much of every softmax), and pages that only hold others are given back.
 """
 from __future__ import annotations
 
@@ -28,6 +31,8 @@ class YvCacheConfig:
     max_blocks_per_seq: int = 2048
     dtype: torch.dtype = torch.bfloat16
     sliding_window: Optional[int] = None      # keep only the last N tokens addressable (opt-in, lossy)
+    attention_window: Optional[int] = None    # tokens attend to the last N tokens, their own included (opt-in, lossy) ...
+    first_tokens: int = 0                     # ... and to the first ones of their sequence
 
 
 class YvBlockAllocator:
@@ -66,20 +71,53 @@ class YvPagedKVCache:
         self.cfg, self.device = cfg, device
         self.n_layer, self.hk, self.d = n_layer, n_kv_head, head_dim
         shape = (cfg.num_blocks, cfg.block_size, n_kv_head, head_dim)
-        self.k = [torch.zeros(shape, dtype=cfg.dtype, device=device) for _ in range(n_layer)]
-        self.v = [torch.zeros(shape, dtype=cfg.dtype, device=device) for _ in range(n_layer)]
+        if cfg.attention_window is not None and (cfg.attention_window < 1 or cfg.first_tokens < 0):
+            raise ValueError(f"a window of {cfg.attention_window} tokens and {cfg.first_tokens} first ones")
+        if cfg.attention_window is None and cfg.first_tokens:
+            raise ValueError("first_tokens are those that stay visible beside an attention_window")
+        if cfg.attention_window is not None and cfg.sliding_window is not None:
+            raise ValueError("attention_window masks keys where they lie, sliding_window moves them: one of the two")
+        self.fp8 = cfg.dtype == torch.float8_e4m3fn
+        page = lambda: torch.zeros(shape, dtype=torch.uint8, device=device).view(cfg.dtype) if self.fp8 else \
+            torch.zeros(shape, dtype=cfg.dtype, device=device)
+        self.k = [page() for _ in range(n_layer)]
+        self.v = [page() for _ in range(n_layer)]
+        scale = lambda: torch.zeros(cfg.num_blocks, n_kv_head, cfg.block_size, dtype=torch.uint8, device=device)
+        self.k_scale = [scale() for _ in range(n_layer)] if self.fp8 else []
+        self.v_scale = [scale() for _ in range(n_layer)] if self.fp8 else []
         self.alloc = YvBlockAllocator(cfg.num_blocks)
         self.tables: Dict[int, List[int]] = {}       # seq id -> physical blocks
         self.lengths: Dict[int, int] = {}
         self.layer_offset = 0                         # first global layer index held by this pipeline stage
         # tokens (the query's own included) that the widest layer still reads; None = every token stays addressable
-        self.reach: Optional[int] = None
+        self.reach: Optional[int] = cfg.attention_window
+
+    @property
+    def pages_only(self) -> bool:
+        """Whether attention has to go through ``ops.cache`` (8-bit pages, or a window over them)."""
+        return self.fp8 or self.cfg.attention_window is not None
+
+    def scales(self, idx: int) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+        """Exponent bytes of a layer's keys and values in 8 bits, else (None, None)."""
+        at = idx - self.layer_offset
+        return (self.k_scale[at], self.v_scale[at]) if self.fp8 else (None, None)
+
+    def read(self, seq_id: int, idx: int, lo: int = 0, hi: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Keys (as rotated at their positions) and values of a sequence's tokens lo .. hi - 1 in one layer [hi - lo, hk * d]: a
+        prefix to hand to another cache, or to look at."""
+        slots = self.slots(seq_id, lo, self.lengths[seq_id] if hi is None else hi)
+        at = torch.from_numpy(slots).to(self.device)
+        k, v = self.layer(idx)
+        if self.fp8:
+            from ..ops import cache as C
+            return C.kv_cache_read_fp8(k, v, *self.scales(idx), at.int())
+        return k.view(-1, self.hk * self.d)[at], v.view(-1, self.hk * self.d)[at]
 
     def layer(self, idx: int) -> Tuple[torch.Tensor, torch.Tensor]:
         return self.k[idx - self.layer_offset], self.v[idx - self.layer_offset]
 
     def bytes(self) -> int:
-        return 2 * self.n_layer * self.k[0].numel() * self.k[0].element_size()
+        return 2 * self.n_layer * self.k[0].numel() * self.k[0].element_size() + sum(t.numel() for t in self.k_scale + self.v_scale)
 
     # ---- sequence management (host) ---------------------------------------------------------------
     def add_sequence(self, seq_id: int) -> None:
@@ -100,8 +138,9 @@ class YvPagedKVCache:
             return 0
         bs, tbl = self.cfg.block_size, self.tables[seq_id]
         last = (self.lengths[seq_id] - self.reach + 1 - bs) // bs          # pages below this one are out of reach
+        kept = -(-self.cfg.first_tokens // bs)                             # pages of the first tokens
         freed = 0
-        for i in range(min(last, len(tbl)) - 1, -1, -1):
+        for i in range(min(last, len(tbl)) - 1, kept - 1, -1):
             if tbl[i] == RELEASED:
                 break                                                     # everything in front of it has gone before
             self.alloc.release(tbl[i])
@@ -162,7 +201,8 @@ class YvPagedKVCache:
     # ---- checkpoint / restore (reference cache.py:2394-2430) ------------------------------------------------
     def state(self) -> Dict[str, object]:
         return {"tables": {k: list(v) for k, v in self.tables.items()}, "lengths": dict(self.lengths),
-                "k": [t.cpu() for t in self.k], "v": [None if t is None else t.cpu() for t in self.v]}
+                "k": [t.cpu() for t in self.k], "v": [None if t is None else t.cpu() for t in self.v],
+                "k_scale": [t.cpu() for t in self.k_scale], "v_scale": [t.cpu() for t in self.v_scale]}
 
     def load_state(self, st: Dict[str, object]) -> None:
         self.tables = {int(k): list(v) for k, v in st["tables"].items()}      # type: ignore[union-attr]
@@ -171,9 +211,14 @@ class YvPagedKVCache:
         self.alloc = YvBlockAllocator(self.cfg.num_blocks)
         self.alloc.free = [b for b in range(self.cfg.num_blocks - 1, -1, -1) if b not in used]
         self.alloc.refs = {b: sum(b in t for t in self.tables.values()) for b in used}
-        for mine, saved in ((self.k, st["k"]), (self.v, st["v"])):
+        for mine, saved in ((self.k, st["k"]), (self.v, st["v"]), (self.k_scale, st.get("k_scale", [])),
+                            (self.v_scale, st.get("v_scale", []))):
+            if len(mine) != len(saved):                                        # type: ignore[arg-type]
+                raise ValueError("the saved cache holds its keys and values in another form")
             for t, src in zip(mine, saved):                                    # type: ignore[arg-type]
                 if t is not None:
+                    if t.dtype != src.dtype and torch.float8_e4m3fn in (t.dtype, src.dtype):
+                        raise ValueError(f"a saved cache of {src.dtype} for one of {t.dtype}")
                     t.copy_(src)
 
 
@@ -182,6 +227,9 @@ class YvPagedLayeredCache(YvPagedKVCache):
     token) or ``{"heads": g, "dim": d, "vdim": e}`` (keys ``[num_blocks, block_size, g, d]`` and values ``[.., g, e]``)."""
 
     def __init__(self, layouts: List[Dict[str, int]], cfg: YvCacheConfig, device: torch.device, reach: Optional[int] = None):
+        if cfg.dtype == torch.float8_e4m3fn or cfg.attention_window is not None:
+            raise ValueError("layered models bring windows of their own and read bf16 or fp32 pages")
+        self.fp8, self.k_scale, self.v_scale = False, [], []
         self.cfg, self.device = cfg, device
         self.n_layer = len(layouts)
         self.hk = max(m.get("heads", 1) for m in layouts)
@@ -209,8 +257,11 @@ class YvPagedLayeredCache(YvPagedKVCache):
 
 
 def cache_for_model(cfg, device: torch.device, num_blocks: int, block_size: Optional[int] = None, tp_size: int = 1,
-                    n_layer: Optional[int] = None, dtype: torch.dtype = torch.bfloat16) -> YvPagedKVCache:
-    cc = YvCacheConfig(block_size=block_size or cfg.kv_cache_block_size, num_blocks=num_blocks, dtype=dtype)
+                    n_layer: Optional[int] = None, dtype: torch.dtype = torch.bfloat16, attention_window: Optional[int] = None,
+                    first_tokens: int = 0) -> YvPagedKVCache:
+    """``dtype`` float8_e4m3fn, ``attention_window`` and ``first_tokens``: see ``YvCacheConfig``."""
+    cc = YvCacheConfig(block_size=block_size or cfg.kv_cache_block_size, num_blocks=num_blocks, dtype=dtype,
+                       attention_window=attention_window, first_tokens=first_tokens)
     if cfg.layer_specs:
         from .registry import cache_layout
         layouts, reach = cache_layout(cfg)

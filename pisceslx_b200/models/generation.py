@@ -172,6 +172,8 @@ def _prefill(model, ids: torch.Tensor, cache: YvPagedKVCache, seq_ids: List[int]
         first = to_device(starts, torch.int32, ids.device)
         ctx.positions = ctx.positions + first.repeat_interleave(S + pad)
         ctx.max_position = max(starts) + S + pad
+        if getattr(trunk, "rotary", None) is not None:
+            ctx.cos, ctx.sin = trunk.rotary.tables(ctx.max_position, ids.device)
     slots: List[int] = []
     for s in seq_ids:
         slots += cache.append_slots(s, S) + [-1] * pad

@@ -21,7 +21,7 @@ import torch.nn as nn
 from ..config import YvConfig
 from ..ops import functional as F_
 from ..ops.loss import linear_cross_entropy, rows_at_once
-from .attention import AttnContext
+from .attention import AttnContext, YvAttention
 from .blocks import YvTransformerBlock
 from .norms import YvRMSNorm, YvRotaryEmbedding
 from .registry import model_class
@@ -202,7 +202,14 @@ class YvModel(YvPackedTrunk):
 
 class YvModelForCausalLM(nn.Module):
     trunk_class: type = YvModel
-    supports_portions = False         # attention of a prompt's later portion over cached earlier ones
+
+    @property
+    def supports_portions(self) -> bool:
+        """Whether a prompt may be continued from the cache at any position: all that a token sees of earlier ones is in the
+        cached keys and values (a state-space branch and the knowledge field look at the prompt as a whole), on one rank."""
+        par, trunk = self.parallel, self.model
+        return (par is None or (par.tp_size == 1 and getattr(par, "cp_size", 1) == 1)) and trunk.subconscious is None and \
+            all(type(blk) is YvTransformerBlock and type(blk.attention) is YvAttention and blk.ssm is None for blk in trunk.layers)
 
     def __init__(self, cfg: YvConfig, parallel=None):
         super().__init__()

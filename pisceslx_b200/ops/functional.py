@@ -387,6 +387,12 @@ def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     return o
 
 
+def rope_(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor, hq: int, hk: int, d: int,
+          rot_dim: int) -> None:
+    """On the GPU: rotate q and k [T, h*d] in place, without a gradient."""
+    _k().rope(q, k, cos, sin, positions, hq, hk, d, rot_dim, False)
+
+
 def rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
                hq: int, hk: int, d: int, rot_dim: int, k_cache: torch.Tensor, v_cache: torch.Tensor, slot_map: torch.Tensor) -> None:
     """On the GPU: rotate q and k [T, h*d] in place and append k and v to the paged caches as ``kv_cache_write`` does."""

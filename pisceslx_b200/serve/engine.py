@@ -56,6 +56,9 @@ class YvEngineConfig:
     status_check_steps: int = 16          # read the kernels' status word every this many decode steps (0 = never)
     prefill_portion: int = 0              # run prompts in portions of at most this many tokens (0 = whole; models
                                           # that continue a prompt from the cache only)
+    kv_cache_dtype: str = "model"         # "model": the model's dtype; "fp8_e4m3": 8-bit keys and values (lossy)
+    attention_window: Optional[int] = None    # tokens attend to the last N tokens and to the first_tokens first ones (lossy); pages
+    first_tokens: int = 0                     # that only hold others are given back
 
 
 class YvInferenceEngine:
@@ -68,8 +71,12 @@ class YvInferenceEngine:
         p = next(model.parameters())
         self.device = p.device
         tp = model.parallel.tp_size if getattr(model, "parallel", None) is not None else 1
+        if self.cfg.kv_cache_dtype not in ("model", "fp8_e4m3"):
+            raise ValueError(f"kv_cache_dtype {self.cfg.kv_cache_dtype!r}: 'model' or 'fp8_e4m3'")
         self.cache: YvPagedKVCache = cache_for_model(model.cfg, self.device, self.cfg.num_blocks, self.cfg.block_size,
-                                                     tp_size=tp, n_layer=len(model.model.layers), dtype=p.dtype)
+                                                     tp_size=tp, n_layer=len(model.model.layers),
+                                                     dtype=torch.float8_e4m3fn if self.cfg.kv_cache_dtype == "fp8_e4m3" else p.dtype,
+                                                     attention_window=self.cfg.attention_window, first_tokens=self.cfg.first_tokens)
         self.cache.layer_offset = model.model.layer_lo
         from .graph_decode import YvDecodeGraphRunner
         self.graph = YvDecodeGraphRunner(model, self.cache, min(self.cfg.max_model_len, self.cfg.graph_max_seq_len),
