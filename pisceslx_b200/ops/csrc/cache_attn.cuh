@@ -400,8 +400,9 @@ __global__ void __launch_bounds__(CacheAttn<D>::kThreads, 1) cache_attn_kernel(c
       const bool valid = tok < p.per_tile && q_tok < it.q_len && (t == 0 || it.second);
       const bool live = tok < p.per_tile && q_tok < it.q_len;                    // the row of a shared tile lives in both halves
       const bool warp_live = __any_sync(0xFFFFFFFFu, live);
-      const int hi = live ? q_tok + it.shift : -1;                               // last visible key
-      const int low = p.window > 0 ? hi - p.window + 1 : 0;                      // first key of the window
+      // last visible key, and the window's first; rows that do not exist are not masked (nobody looks at them)
+      const int hi = live ? q_tok + it.shift : 0x7FFFFFFF;
+      const int low = live && p.window > 0 ? hi - p.window + 1 : 0;
       float m_used = -1.0e29f;                        // running maximum (log2 domain); above kCaMask, so masked scores give 0
       float l_sum = 0.f;
       for (int j = 0; j < n_kv && ok; ++j, ++ns) {
@@ -423,11 +424,16 @@ __global__ void __launch_bounds__(CacheAttn<D>::kThreads, 1) cache_attn_kernel(c
             tmem_ld32(tS + 96, c3);
             tc_wait_ld();
           }
-          if (key0 + kCaTile - 1 > hi || (key0 < low && key0 + kCaTile > p.first)) {
-            const int end = hi - key0, from = low - key0, head = p.window > 0 ? p.first - key0 : 0;
+          if (__any_sync(0xFFFFFFFFu, key0 + kCaTile - 1 > hi || (key0 < low && key0 + kCaTile > p.first))) {
+            // a bit for each visible key (compared one by one, with branches, a masked tile took 13000 cycles)
+            const int end = hi - key0, from = low - key0, head = p.first - key0;
 #pragma unroll
-            for (int i = 0; i < 128; ++i)
-              if (i > end || (i < from && i >= head)) sreg[i] = 0xFF800000u;     // -inf: 2^(-inf) = 0
+            for (int w = 0; w < 4; ++w) {
+              auto below = [&](int n) { return n <= 32 * w ? 0u : n >= 32 * w + 32 ? 0xFFFFFFFFu : (1u << (n - 32 * w)) - 1u; };
+              const uint32_t bits = (end >= 127 ? 0xFFFFFFFFu : below(end + 1)) & (~below(from) | below(head));
+#pragma unroll
+              for (int i = 0; i < 32; ++i) sreg[32 * w + i] = (bits >> i) & 1u ? sreg[32 * w + i] : 0xFF800000u;      // -inf: 2^(-inf) = 0
+            }
           }
           float m4[4] = {kCaMask, kCaMask, kCaMask, kCaMask};
 #pragma unroll
@@ -444,7 +450,7 @@ __global__ void __launch_bounds__(CacheAttn<D>::kThreads, 1) cache_attn_kernel(c
           if (!(mx <= m_used + kCaRescale)) {         // lazy: the reference maximum moves in large steps only
             alpha = exp2f(m_used - mx);
             m_used = mx;
-            rescale = (j > 0);
+            rescale = (j > 0) && live;
           }
           if (__any_sync(0xFFFFFFFFu, rescale)) {
             // O holds sums relative to the old maximum; the products that wrote it precede the scores just read

@@ -703,7 +703,8 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
 #pragma unroll
           for (int i = 0; i < C; ++i) {
             const int hi = sHi[tb * N + n0 + i];
-            if (!(seen && key <= hi && (p.window == 0 || key > hi - p.window || key < p.first))) sc[i] = kCaMask;
+            const bool mine = seen & (key <= hi) & ((p.window == 0) | (key > hi - p.window) | (key < p.first));
+            sc[i] = mine ? sc[i] : kCaMask;
           }
         }
       };
