@@ -19,6 +19,8 @@ namespace {
 constexpr int kRowsThreads = 256;
 
 // One group of d / 8 lanes per row: 16 bytes in, 8 bytes of codes out, a byte by the first lane.
+// Bound by bytes: 8191 tokens of 8 heads of 128 (50 MB) take 19 us from a cold cache, a copy of as many bytes 22.6; two or four rows
+// a group, loaded ahead, 20.5.
 template <int D, bool CHAIN>
 __global__ void __launch_bounds__(kRowsThreads) cache_write_fp8_kernel(const CacheRowsArgs a) {
   constexpr int kLanes = D / 8;
@@ -228,6 +230,13 @@ int page_map(CUtensorMap* m, const CacheAttnArgs& a, const void* pages, int64_t 
 
 namespace {
 
+// Key ranges of a block: the number that takes the least time, by an estimate in us: 1.9 a step (D = 128) and 2 a range for each
+// round of ranges over the SMs, 2 for the second kernel and its bytes at 3 TB/s (a fit to 17 calls: (new tokens of cached) 512 of
+// 16384, 32 heads over 8, D = 128: one range 256 us, two 154, three 201, eight 184; 128 of 16384: 250, 141, 104, 57; 2048 of 32768:
+// 971, 1051, 1079, 1164.  The estimate's choice was within 5 % of the best of 12 numbers in 15 of the calls, 26 % off at worst).
+// Equal pieces of one line of all tiles, as in cache_few.cuh, balance better but lose: 166 for the first call and 1908 for 4096 of
+// 32768, where ranges take 154 and 1740.  Blocks of one head that walk the same keys at the same time share them in the L2; pieces
+// begin anywhere, and each tile then comes from far away or from DRAM (2.7 GB read where the cache holds 0.13).
 int tile_splits(const CacheAttnArgs& a) {
   const CacheGrid g = cache_grid(a);
   const int sms = sm_count();
@@ -236,10 +245,12 @@ int tile_splits(const CacheAttnArgs& a) {
   // steps of an item: key tiles of a block of two query tiles, pairs of key tiles of a lone one
   const double steps = static_cast<double>((keys + kCaTile - 1) / kCaTile) / (g.two ? 1 : 2);
   const int64_t room = (int64_t(256) << 20) / (a.total_q * a.hq * a.d * 4 + 1);              // ranges that the scratch has room for
+  const double sums = static_cast<double>(a.total_q) * a.hq * a.d * 8;                       // bytes written and read, per range
   int best = 1;
   double least = 0;
   for (int s = 1; s <= 32 && (s == 1 || (s <= 2 * steps && s <= room)); ++s) {
-    const double cost = static_cast<double>((g.items * s + sms - 1) / sms) * (steps / s + 2) + (s > 1 ? 3 + 0.1 * s : 0);
+    const double rounds = static_cast<double>((g.items * s + sms - 1) / sms);
+    const double cost = rounds * (steps / s * 1.9 + 2) + (s > 1 ? 2 + s * sums / 3e6 : 0);
     if (s == 1 || cost < least) { best = s; least = cost; }
   }
   return best;
