@@ -64,6 +64,9 @@ struct CacheFew {
   // their own (an even number); else, in the order of the ring, by the product with the values.  A copying warp that waits for a
   // stage must not see it given back a turn too early.
   static constexpr bool kEarly = F8 && kStages % 2 == 0;
+  // From 32 rows on the softmax warps make codes of their own item's query rows: one warp that does it for both pieces takes 8000
+  // cycles for 64 rows, and an item's first scores wait for it.  Of few rows it is done ahead.
+  static constexpr bool kOwnRows = F8 && R >= 32;
   static constexpr int kTotal = kFixed + kStages * kStage + kRest + 1024;
   static constexpr uint32_t kSCols = F8 ? 2 * kN : kN;               // columns of a score buffer
   static constexpr uint32_t kUsed = 2 * kSCols + 2 * kN;             // scores and sums of two pieces
@@ -71,8 +74,18 @@ struct CacheFew {
   static_assert(kStages >= 2 && kTotal <= 227 * 1024 && kUsed <= 512, "room");
 };
 
-// Places of the line in front of piece c of n.
-__device__ __forceinline__ int few_cut(int all, int c, int n) { return static_cast<int>(static_cast<int64_t>(all) * c / n); }
+// The line in n pieces: the first `more` have a tile more than the others (32-bit arithmetic and one division: every warp asks
+// before it can begin).
+struct CacheFewCuts {
+  int each, more, n;
+  __device__ __forceinline__ CacheFewCuts(int all, int n_) : each(all / n_), more(all - all / n_ * n_), n(n_) {}
+  __device__ __forceinline__ int cut(int c) const { return c < n ? each * c + min(c, more) : each * n + more; }    // places in front of piece c
+  __device__ __forceinline__ int tiles(int c) const { return c < n ? each + (c < more ? 1 : 0) : 0; }
+  __device__ __forceinline__ int piece(int x) const {
+    const int longer = (each + 1) * more;
+    return x < longer ? x / (each + 1) : more + (x - longer) / each;
+  }
+};
 __device__ __forceinline__ int few_pieces(int all, int ctas) {
   return all >= 2 * kFewTwo * ctas ? 2 * ctas : max(1, min(ctas, all / kFewLeast));
 }
@@ -90,10 +103,9 @@ struct CacheFewItem : CacheTiles {
   int b, kvh, q_begin, q_len, shift, n;
   int slot;                          // -1: whole, else which of the piece's parts
 
-  __device__ __forceinline__ void begin_walk(const CacheAttnParams& p, const CacheFewTable& t, int pieces, int piece) {
-    const int all = t.pre[p.batch] * p.hk;
-    start = at = few_cut(all, min(piece, pieces), pieces);
-    end = few_cut(all, min(piece + 1, pieces), pieces);
+  __device__ __forceinline__ void begin_walk(const CacheAttnParams& p, const CacheFewTable& t, const CacheFewCuts& cuts, int piece) {
+    start = at = cuts.cut(piece);
+    end = start + cuts.tiles(piece);
     int low = 0, high = p.batch;     // the last sequence with pre <= at / hk
     while (high - low > 1) {
       const int mid = (low + high) / 2;
@@ -230,6 +242,54 @@ __device__ __forceinline__ float few_power(uint32_t byte) {
   return byte == 255u ? __int_as_float(0x7FC00000) : byte == 0u ? __int_as_float(0x00400000) : __int_as_float(static_cast<int>(byte) << 23);
 }
 
+// Query rows (bf16, as they lie) to two codes for each number and a power of two for each row: codes of what is left after the first
+// ones, times 16, are rows N + i.  Four lanes for a row, eight rows at a time for a warp; `rows`: the table of rows, -1 = none.
+template <int D, int N, int R>
+__device__ __forceinline__ void few_query(const uint8_t* raw, uint8_t* dst, float* factor, const int* rows, float scale, int from, int step) {
+  const int part = threadIdx.x & 3;
+#pragma unroll 1
+  for (int i = from + ((threadIdx.x & 31) >> 2); i < (R < 8 ? 8 : R); i += step) {
+    const bool there = i < R && rows[i] >= 0;
+    constexpr int kVecs = D / 32;                                    // 16-byte vectors of a lane
+    uint4 x[kVecs];
+    uint32_t m2 = 0;
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) {
+      x[v] = there ? *reinterpret_cast<const uint4*>(raw + i * D * 2 + (part * kVecs + v) * 16) : make_uint4(0, 0, 0, 0);
+      m2 = __vmaxu2(__vmaxu2(m2, x[v].x & 0x7FFF7FFFu), __vmaxu2(x[v].y & 0x7FFF7FFFu, __vmaxu2(x[v].z & 0x7FFF7FFFu, x[v].w & 0x7FFF7FFFu)));
+    }
+    uint32_t most = max(m2 & 0xFFFFu, m2 >> 16);
+    most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
+    most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
+    const bool finite = most < 0x7F80u;
+    const int byte = finite ? max(0, static_cast<int>(most >> 7) - 8 + ((most & 0x7Fu) > 0x60u ? 1 : 0)) : 127;
+    const float inv = __int_as_float((254 - byte) << 23);            // 2^-E
+#pragma unroll
+    for (int v = 0; v < kVecs; v += 2) {
+      const uint32_t w[8] = {x[v].x, x[v].y, x[v].z, x[v].w, x[v + 1].x, x[v + 1].y, x[v + 1].z, x[v + 1].w};
+      uint32_t c1[4] = {0, 0, 0, 0}, c2[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float2 f = make_float2(__uint_as_float(w[e] << 16) * inv, __uint_as_float(w[e] & 0xFFFF0000u) * inv);
+        const __nv_fp8x2_storage_t a = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
+        const float2 y = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(a, __NV_E4M3)));
+        const __nv_fp8x2_storage_t b = __nv_cvt_float2_to_fp8x2(make_float2((f.x - y.x) * 16.f, (f.y - y.y) * 16.f), __NV_SATFINITE, __NV_E4M3);
+        c1[e / 2] |= static_cast<uint32_t>(a) << (16 * (e & 1));
+        c2[e / 2] |= static_cast<uint32_t>(b) << (16 * (e & 1));
+      }
+      // rows i and N + i (N is a multiple of 16: the same exchange of places)
+      const int at = few_place<D>(i, (part * kVecs + v) / 2) << 4;
+      if (i < R) {
+        *reinterpret_cast<uint4*>(dst + i * D + at) = finite ? make_uint4(c1[0], c1[1], c1[2], c1[3]) : make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(dst + (N + i) * D + at) = finite ? make_uint4(c2[0], c2[1], c2[2], c2[3]) : make_uint4(0, 0, 0, 0);
+      }
+    }
+    if (part == 0 && i < R) factor[i] = finite ? scale * few_power(byte) : __int_as_float(0x7FC00000);
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
 // Barrier over `THREADS` threads with an OR of `v` (lanes that left a wait at different times are brought together first).
 template <int THREADS>
 __device__ __forceinline__ bool few_any(int id, bool v) {
@@ -279,8 +339,9 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
   uint64_t* q_empty = v_full + 2;            // [2] query rows
   uint64_t* q_full = q_empty + 2;            // [2][2] query rows and their tables, of which there are two
   uint64_t* t_empty = q_full + 4;            // [2][2]
-  uint64_t* raw_full = t_empty + 4;          // query rows as they were
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(raw_full + 1);
+  uint64_t* raw_full = t_empty + 4;          // [2] query rows as they were (of a piece: kOwnRows)
+  uint64_t* raw_empty = raw_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(raw_empty + 1);
   uint8_t* sByte = reinterpret_cast<uint8_t*>(bars) + 256;                               // [kStages][2][128]
   CacheFewTile* sTile = reinterpret_cast<CacheFewTile*>(sByte + kStages * 2 * kCaTile);  // [kStages]
   volatile int* sFirst = reinterpret_cast<int*>(bars) + 60;                              // [2] whether the weights are an item's first
@@ -315,9 +376,11 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
       mbar_init(&v_full[i], 4);
       mbar_init(&q_empty[i], 1);
     }
-    mbar_init(raw_full, 1);
+    mbar_init(&raw_full[0], 1);
+    mbar_init(&raw_full[1], 1);
+    mbar_init(raw_empty, 4);
     for (int i = 0; i < 4; ++i) {
-      mbar_init(&q_full[i], F8 ? 1 : 2);     // the tables, and where they are copied as they are the rows
+      mbar_init(&q_full[i], !F8 ? 2 : S::kOwnRows ? 4 : 1);     // the rows, and the tables where those are copied as they are
       mbar_init(&t_empty[i], 4);
     }
     fence_barrier_init();
@@ -366,8 +429,7 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
     int* totals = reinterpret_cast<int*>(sRed);                      // [warps]
     if (lane == 31) totals[warp] = scan;
     __syncthreads();
-    int ahead = scan - sum;
-    for (int w = 0; w < warp; ++w) ahead += totals[w];
+    int ahead = scan - sum + __reduce_add_sync(0xFFFFFFFFu, lane < warp ? totals[lane] : 0);
     for (int b = b0; b < b1; ++b) {
       ahead += tab.pre[b + 1];
       tab.pre[b + 1] = ahead;
@@ -377,87 +439,91 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
   }
   if (blockIdx.x == 0)
     for (int b = tid; b <= p.batch; b += S::kThreads) fp.pre[b] = tab.pre[b];
-  const int pieces = few_pieces(tab.pre[p.batch] * p.hk, gridDim.x);
+  const int places = tab.pre[p.batch] * p.hk;
+  const CacheFewCuts cuts(places, few_pieces(places, gridDim.x));
 
   auto stage_v = [&](uint32_t s) { return sRing + s * S::kStage; };
   auto stage_k = [&](uint32_t s) { return sRing + s * S::kStage + S::kHalf; };
   const uint32_t tO = tmem_base + 2 * S::kSCols;                     // [2] of N columns behind the scores
 
-  // tiles of both pieces
-  const int places = tab.pre[p.batch] * p.hk;
-  auto tiles_of = [&](int piece) { return few_cut(places, min(piece + 1, pieces), pieces) - few_cut(places, min(piece, pieces), pieces); };
   // the longer one is the first
-  const int extra = tiles_of(gridDim.x + blockIdx.x) > tiles_of(blockIdx.x) ? 1 : 0;
+  const int extra = cuts.tiles(gridDim.x + blockIdx.x) > cuts.tiles(blockIdx.x) ? 1 : 0;
   auto piece_of = [&](uint32_t group) { return static_cast<int>(blockIdx.x + ((group ^ extra) != 0u ? gridDim.x : 0u)); };
-  const int both = tiles_of(piece_of(0)) + tiles_of(piece_of(1));
+  const int both = cuts.tiles(piece_of(0)) + cuts.tiles(piece_of(1));       // tiles of both pieces
 
   if (warp == 10 || warp == 11) {
     // ------------------------------------ copies --------------------------------------------
     const uint32_t grp = warp - 10, lead = elect_one() ? 1u : 0u;
     const int piece = piece_of(grp), boxes = kCaTile / p.box, per_look = 32 / boxes;
-    const uint32_t others = both - tiles_of(piece);
+    const uint32_t others = both - cuts.tiles(piece);
     uint32_t k = 0;
     bool ok = true;
     CacheFewItem it;
-    it.begin_walk(p, tab, pieces, piece);
+    it.begin_walk(p, tab, cuts, piece);
     while (ok && it.next(p, tab)) {
+      // lane i: slot of copy i of the next tiles and its place in the page (negative where no key of it is seen), looked up while
+      // those of the tiles in front are used; a lone place for it, so that its code is there once
       int2 rows = {}, next = {};
-      for (int j = 0, in = per_look; j < it.n; ++j, ++k) {
-        // lane i: slot of copy i of the next tiles and its place in the page (negative where no key of it is seen), looked up ahead
-        for (; in == per_look; in = 0) {
-          for (int ahead = j == 0 ? 0 : per_look; ahead <= per_look; ahead += per_look) {
-            const int at = j + ahead + lane / boxes, key = it.first_key(at) + (lane % boxes) * p.box;
-            rows = next;
-            next = at < it.n && it.any(key, p.box) ? make_int2(ca_slot(p, it.b, key), key % p.block) : make_int2(-1, 0);
+      for (int j = -1, in = per_look - 1; j < it.n; ++j) {
+        const bool look = ++in == per_look;
+        if (look) {
+          if (j >= 0) in = 0;
+          rows = next;
+        }
+        if (j >= 0) {
+          const uint32_t g = few_turn(k, grp, others), s = g % kStages;
+          const uint32_t here = __ballot_sync(0xFFFFFFFFu, rows.x >= 0 && lane / boxes == in);
+          ok = few_wait_warp(&empty[s], ((g / kStages) & 1u) ^ 1u, p.status);
+          if (!ok) break;
+          if (lead) {
+            const int key0 = it.first_key(j);
+            const bool whole = it.whole(key0);
+            const bool all = whole && key0 + kCaTile - 1 <= it.shift &&
+                             (p.window == 0 || key0 > it.q_len - 1 + it.shift - p.window || key0 + kCaTile <= p.first);
+            sTile[s].key = key0;
+            sTile[s].flags = static_cast<int>(grp) | (j == 0 ? kFewFirst : 0) | (j + 1 == it.n ? kFewLast : 0) | (whole ? kFewWhole : 0) |
+                             (all ? kFewAll : 0);
+            sTile[s].lo = it.lo;
+            sTile[s].last = it.last;
+            sTile[s].first_end = it.first_end;
+            mbar_expect_tx(&full[s], static_cast<uint32_t>(__popc(here)) * p.box * (F8 ? 2 * D + 2 : 4 * D));
           }
-        }
-        const uint32_t g = few_turn(k, grp, others), s = g % kStages;
-        const uint32_t here = __ballot_sync(0xFFFFFFFFu, rows.x >= 0 && lane / boxes == in);
-        ok = few_wait_warp(&empty[s], ((g / kStages) & 1u) ^ 1u, p.status);
-        if (!ok) break;
-        if (lead) {
-          const int key0 = it.first_key(j);
-          const bool whole = it.whole(key0);
-          const bool all = whole && key0 + kCaTile - 1 <= it.shift &&
-                           (p.window == 0 || key0 > it.q_len - 1 + it.shift - p.window || key0 + kCaTile <= p.first);
-          sTile[s].key = key0;
-          sTile[s].flags = static_cast<int>(grp) | (j == 0 ? kFewFirst : 0) | (j + 1 == it.n ? kFewLast : 0) | (whole ? kFewWhole : 0) |
-                           (all ? kFewAll : 0);
-          sTile[s].lo = it.lo;
-          sTile[s].last = it.last;
-          sTile[s].first_end = it.first_end;
-          mbar_expect_tx(&full[s], static_cast<uint32_t>(__popc(here)) * p.box * (F8 ? 2 * D + 2 : 4 * D));
-        }
-        for (int i = 0; i < boxes; ++i) {
-          const int row = __shfl_sync(0xFFFFFFFFu, rows.x, in * boxes + i), off = __shfl_sync(0xFFFFFFFFu, rows.y, in * boxes + i);
-          if (!lead || row < 0) continue;
-          if constexpr (F8) {
-            const int64_t from = static_cast<int64_t>(row) * p.hk + it.kvh * p.block - off * (p.hk - 1);   // [page][head][place]
-            tma_load_3d(stage_k(s) + i * p.box * D, &fp.tma_k, &full[s], 0, it.kvh, row);
-            bulk_load_1d(sByte + s * 2 * kCaTile + i * p.box, fp.ks + from, p.box, &full[s]);
-            tma_load_3d(stage_v(s) + i * p.box * D, &fp.tma_v, &full[s], 0, it.kvh, row);
-            bulk_load_1d(sByte + s * 2 * kCaTile + kCaTile + i * p.box, fp.vs + from, p.box, &full[s]);
-          } else {
+          for (int i = 0; i < boxes; ++i) {
+            const int row = __shfl_sync(0xFFFFFFFFu, rows.x, in * boxes + i), off = __shfl_sync(0xFFFFFFFFu, rows.y, in * boxes + i);
+            if (!lead || row < 0) continue;
+            if constexpr (F8) {
+              const int64_t from = static_cast<int64_t>(row) * p.hk + it.kvh * p.block - off * (p.hk - 1);   // [page][head][place]
+              tma_load_3d(stage_k(s) + i * p.box * D, &fp.tma_k, &full[s], 0, it.kvh, row);
+              bulk_load_1d(sByte + s * 2 * kCaTile + i * p.box, fp.ks + from, p.box, &full[s]);
+              tma_load_3d(stage_v(s) + i * p.box * D, &fp.tma_v, &full[s], 0, it.kvh, row);
+              bulk_load_1d(sByte + s * 2 * kCaTile + kCaTile + i * p.box, fp.vs + from, p.box, &full[s]);
+            } else {
 #pragma unroll
-            for (int c = 0; c < D / 64; ++c) tma_load_3d(stage_k(s) + c * kSlab + i * p.box * 128, &fp.tma_k, &full[s], c * 64, it.kvh, row);
+              for (int c = 0; c < D / 64; ++c) tma_load_3d(stage_k(s) + c * kSlab + i * p.box * 128, &fp.tma_k, &full[s], c * 64, it.kvh, row);
 #pragma unroll
-            for (int c = 0; c < D / 64; ++c) tma_load_3d(stage_v(s) + c * kSlab + i * p.box * 128, &fp.tma_v, &full[s], c * 64, it.kvh, row);
+              for (int c = 0; c < D / 64; ++c) tma_load_3d(stage_v(s) + c * kSlab + i * p.box * 128, &fp.tma_v, &full[s], c * 64, it.kvh, row);
+            }
           }
+          __syncwarp();
+          ++k;
         }
-        __syncwarp();
-        ++in;
+        if (look) {
+          const int at = (j < 0 ? 0 : j + per_look) + lane / boxes, key = it.first_key(at) + (lane % boxes) * p.box;
+          next = at < it.n && it.any(key, p.box) ? make_int2(ca_slot(p, it.b, key), key % p.block) : make_int2(-1, 0);
+          if (j < 0) in = per_look - 1;
+        }
       }
     }
   } else if (warp == 9) {
     // ------------------------------------ query rows ----------------------------------------
     // Items of both pieces, in the order in which their first tiles are multiplied.
-    const int n0 = tiles_of(piece_of(0));
+    const int n0 = cuts.tiles(piece_of(0));
     const uint32_t lead = elect_one() ? 1u : 0u;
     uint32_t items[2] = {0u, 0u}, k[2] = {0u, 0u}, fills = 0;        // items and tiles so far, copies of query rows
     CacheFewItem now, then;
     uint32_t grp = 0;
-    now.begin_walk(p, tab, pieces, piece_of(0));
-    then.begin_walk(p, tab, pieces, piece_of(1));
+    now.begin_walk(p, tab, cuts, piece_of(0));
+    then.begin_walk(p, tab, cuts, piece_of(1));
     for (;;) {
       const uint32_t turn0 = few_turn(k[0], 0, both - n0), turn1 = few_turn(k[1], 1, n0);
       const bool live0 = k[0] < static_cast<uint32_t>(n0), live1 = k[1] < static_cast<uint32_t>(both - n0);
@@ -473,83 +539,43 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
       it.next(p, tab);
       const uint32_t item = grp != 0 ? items[1] : items[0], tb = grp * 2 + (item & 1u);
       if (!few_wait_warp(&q_empty[grp], (item & 1u) ^ 1u, p.status) || !few_wait_warp(&t_empty[tb], ((item >> 1) & 1u) ^ 1u, p.status)) break;
-      const int box = p.group * p.per_tile;                          // rows of the copy
-      if constexpr (F8) {
-        if (lead) {
-          mbar_expect_tx(raw_full, static_cast<uint32_t>(box) * D * 2);
-          tma_load_3d(sRaw, &fp.tma_q, raw_full, 0, it.kvh * p.group, it.q_begin);
-        }
-      } else if (lead) {
-        mbar_expect_tx(&q_full[tb], static_cast<uint32_t>(box) * D * 2);
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c)
-          tma_load_3d(sQ + grp * S::kQ + c * (N * 128), &fp.tma_q, &q_full[tb], c * 64, it.kvh * p.group, it.q_begin);
-      }
-      __syncwarp();
       if (lane == 0) sItem[tb] = make_int4(it.q_begin, it.kvh, it.slot, 0);
       for (int i = lane; i < R; i += 32) {
         const int tok = i / p.group;
         sHi[tb * N + i] = tok < it.q_len ? tok + it.shift : -1;
         sRow[tb * N + i] = tok < it.q_len ? tok << 8 | (i - tok * p.group) : -1;
       }
-      if constexpr (F8) {
-        // Four lanes for a row, eight rows at a time: the row's power of two, and two codes for each number.
-        if (!few_wait_warp(raw_full, fills & 1u, p.status)) break;
-        ++fills;
-        uint8_t* dst = sQ + grp * S::kQ;
-        const int part = lane & 3;
-#pragma unroll 1
-        for (int i = lane >> 2; i < (R < 8 ? 8 : R); i += 8) {
-          const bool there = i / p.group < it.q_len && i < R;
-          constexpr int kVecs = D / 32;                              // 16-byte vectors of a lane
-          uint4 x[kVecs];
-          uint32_t m2 = 0;
-#pragma unroll
-          for (int v = 0; v < kVecs; ++v) {
-            x[v] = there ? *reinterpret_cast<const uint4*>(sRaw + i * D * 2 + (part * kVecs + v) * 16) : make_uint4(0, 0, 0, 0);
-            m2 = __vmaxu2(__vmaxu2(m2, x[v].x & 0x7FFF7FFFu), __vmaxu2(x[v].y & 0x7FFF7FFFu, __vmaxu2(x[v].z & 0x7FFF7FFFu, x[v].w & 0x7FFF7FFFu)));
-          }
-          uint32_t most = max(m2 & 0xFFFFu, m2 >> 16);
-          most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
-          most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
-          const bool finite = most < 0x7F80u;
-          const int byte = finite ? max(0, static_cast<int>(most >> 7) - 8 + ((most & 0x7Fu) > 0x60u ? 1 : 0)) : 127;
-          const float inv = __int_as_float((254 - byte) << 23);      // 2^-E
-#pragma unroll
-          for (int v = 0; v < kVecs; v += 2) {
-            const uint32_t w[8] = {x[v].x, x[v].y, x[v].z, x[v].w, x[v + 1].x, x[v + 1].y, x[v + 1].z, x[v + 1].w};
-            uint32_t c1[4] = {0, 0, 0, 0}, c2[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float2 f = make_float2(__uint_as_float(w[e] << 16) * inv, __uint_as_float(w[e] & 0xFFFF0000u) * inv);
-              const __nv_fp8x2_storage_t a = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
-              const float2 y = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(a, __NV_E4M3)));
-              const __nv_fp8x2_storage_t b =
-                  __nv_cvt_float2_to_fp8x2(make_float2((f.x - y.x) * 16.f, (f.y - y.y) * 16.f), __NV_SATFINITE, __NV_E4M3);
-              c1[e / 2] |= static_cast<uint32_t>(a) << (16 * (e & 1));
-              c2[e / 2] |= static_cast<uint32_t>(b) << (16 * (e & 1));
-            }
-            // rows i and N + i (N is a multiple of 16: the same exchange of places)
-            const int at = few_place<D>(i, (part * kVecs + v) / 2) << 4;
-            if (i < R) {
-              *reinterpret_cast<uint4*>(dst + i * D + at) = finite ? make_uint4(c1[0], c1[1], c1[2], c1[3]) : make_uint4(0, 0, 0, 0);
-              *reinterpret_cast<uint4*>(dst + (N + i) * D + at) = finite ? make_uint4(c2[0], c2[1], c2[2], c2[3]) : make_uint4(0, 0, 0, 0);
-            }
-          }
-          if (part == 0 && i < R)
-            sFactor[tb * N + i] = finite ? p.scale_log2 * few_power(byte) : __int_as_float(0x7FC00000);
-        }
-        fence_proxy_async_smem();
-      }
       __syncwarp();
-      // (of bf16 pages the copy's arrival is announced above: this one is the tables')
-      if (lane == 0) mbar_arrive(&q_full[tb]);
+      const int box = p.group * p.per_tile;                          // rows of the copy
+      if constexpr (F8) {
+        uint64_t* raw = &raw_full[S::kOwnRows ? grp : 0];
+        if (S::kOwnRows && !few_wait_warp(raw_empty, (fills & 1u) ^ 1u, p.status)) break;
+        if (lead) {
+          mbar_expect_tx(raw, static_cast<uint32_t>(box) * D * 2);
+          tma_load_3d(sRaw, &fp.tma_q, raw, 0, it.kvh * p.group, it.q_begin);
+        }
+        if (!S::kOwnRows) {
+          if (!few_wait_warp(raw, fills & 1u, p.status)) break;
+          few_query<D, N, R>(sRaw, sQ + grp * S::kQ, sFactor + tb * N, sRow + tb * N, p.scale_log2, 0, 8);
+          if (lane == 0) mbar_arrive(&q_full[tb]);
+        }
+        ++fills;
+      } else {
+        if (lead) {
+          mbar_expect_tx(&q_full[tb], static_cast<uint32_t>(box) * D * 2);
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c)
+            tma_load_3d(sQ + grp * S::kQ + c * (N * 128), &fp.tma_q, &q_full[tb], c * 64, it.kvh * p.group, it.q_begin);
+        }
+        // the copy's arrival is announced above: this one is the tables'
+        if (lane == 0) mbar_arrive(&q_full[tb]);
+      }
       if (grp != 0) { ++items[1]; k[1] += it.n; } else { ++items[0]; k[0] += it.n; }
     }
   } else if (warp == 8) {
     // ------------------------------------ products ------------------------------------------
     if (elect_one()) {
-      const uint32_t n0 = tiles_of(piece_of(0)), n1 = both - n0;
+      const uint32_t n0 = cuts.tiles(piece_of(0)), n1 = both - n0;
       uint32_t items0 = 0, items1 = 0;
       // scores of tile k of a piece
       auto scores = [&](uint32_t i, uint32_t k) -> bool {
@@ -608,14 +634,14 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
   } else if (warp >= 12) {
     if constexpr (F8) {
       // ------------------------------------ values to fp16 ----------------------------------
-    constexpr int kLanes = D / 16;                                   // lanes of a row, 16 codes each
-    constexpr int kStep = 128 / kLanes, kRows = kCaTile / kStep;
-    const int c = (tid - 384) % kLanes, row0 = (tid - 384) / kLanes;
-    // 16 codes fill two 16-byte places of a swizzled row.  Where 8 lanes work on one row, those of the second slab start with the
-    // odd place: the 8 stores then meet 8 different groups of banks.  kStep is a multiple of 8: a thread's rows are all alike.
-    const int w = (2 * c) & 7, odd_first = D == 128 && c >= 4 ? 1 : 0;
-    const uint32_t place0 = (c / 4) * kSlab + row0 * 128 + (((w + odd_first) ^ (row0 & 7)) << 4);
-    const uint32_t place1 = (c / 4) * kSlab + row0 * 128 + (((w + 1 - odd_first) ^ (row0 & 7)) << 4);
+      constexpr int kLanes = D / 16;                                   // lanes of a row, 16 codes each
+      constexpr int kStep = 128 / kLanes, kRows = kCaTile / kStep;
+      const int c = (tid - 384) % kLanes, row0 = (tid - 384) / kLanes;
+      // 16 codes fill two 16-byte places of a swizzled row.  Where 8 lanes work on one row, those of the second slab start with the
+      // odd place: the 8 stores then meet 8 different groups of banks.  kStep is a multiple of 8: a thread's rows are all alike.
+      const int w = (2 * c) & 7, odd_first = D == 128 && c >= 4 ? 1 : 0;
+      const uint32_t place0 = (c / 4) * kSlab + row0 * 128 + (((w + odd_first) ^ (row0 & 7)) << 4);
+      const uint32_t place1 = (c / 4) * kSlab + row0 * 128 + (((w + 1 - odd_first) ^ (row0 & 7)) << 4);
       uint32_t k0 = 0, k1 = 0, s = 0, ph = 0;                        // tiles of the pieces
       for (int g = 0; g < both; ++g) {
         if (!few_wait_warp(&full[s], ph, p.status)) break;
@@ -661,12 +687,72 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
     uint32_t k = 0, items = 0;                                       // tiles and items so far
     bool ok = true;
     const int piece = piece_of(grp);
-    const uint32_t mine = tiles_of(piece), others = both - mine;
+    const uint32_t mine = cuts.tiles(piece), others = both - mine;
     constexpr int C = R < 16 ? R : 16;                               // rows at a time
     float* sums = sSum + (grp * 4 + (warp & 3)) * N;
     const int my_row = lane / (32 / C);                              // whose joined value this lane holds
     const bool my_turn = lane % (32 / C) == 0;
-    for (; k < mine; ++k) {
+    bool pending = false;                                            // an item's tiles are done, its sums not yet written
+    for (;; ++k) {
+      if (S::kOwnRows && (k == 0 || pending) && k < mine) {          // before the sums are written: the next scores wait for it
+        const uint32_t next = items + (pending ? 1u : 0u), tb = grp * 2 + (next & 1u);
+        ok = ok && few_wait_warp(&raw_full[grp], next & 1u, p.status);
+        if (ok) {
+          few_query<D, N, R>(sRaw, sQ + grp * S::kQ, sFactor + tb * N, sRow + tb * N, p.scale_log2, (warp & 3) * 8, 32);
+          if (lane == 0) {
+            mbar_arrive(raw_empty);
+            mbar_arrive(&q_full[tb]);
+          }
+        }
+      }
+      if (pending) {
+        const uint32_t tb = grp * 2 + (items & 1u);
+        // ---- the end of an item
+        ok = ok && few_wait(&pv_done[grp], (k - 1u) & 1u, p.status);
+        ok = !few_any<128>(bar, !ok);                // all sums are there
+        if (!ok) break;                              // a wait ran out (the status word says so): the outputs are not written
+        tc_fence_after_sync();
+        const int4 item = sItem[tb];                 // first row of q, key head, slot
+        ++items;
+        const float back = F8 ? few_power(max(top[7], 0)) * 0.0625f : 1.f;                 // 2^(Eref - 4)
+        const float* all = sSum + grp * 4 * N;
+        // a row's factor, for rows of parts with its sum beside it, where the maxima of the warps were
+        if (t < R) {
+          const float sum = (all[t] + all[N + t]) + (all[2 * N + t] + all[3 * N + t]);
+          red[t] = item.z >= 0 ? back : sum > 0.f ? back / sum : sum * 0.f;          // no visible key: 0, NaN stays
+          if (item.z >= 0 && sRow[tb * N + t] >= 0)
+            *reinterpret_cast<float2*>(p.pml + ((static_cast<int64_t>(piece) * 2 + item.z) * R + t) * 2) = make_float2(m_mine[t], sum);
+        }
+        few_any<128>(bar, false);
+        float* part = p.po + (static_cast<int64_t>(piece) * 2 + item.z) * R * D + t;
+        __nv_bfloat16* out = p.o + item.x * p.o_ld + static_cast<int64_t>(item.y * p.group) * D + t;
+#pragma unroll 1
+        for (int n0 = 0; n0 < R; n0 += C) {
+          uint32_t o[16];
+          tmem_ld16(to + n0, o);
+          tc_wait_ld();
+          float f[C];
+          int at[C];
+#pragma unroll
+          for (int i = 0; i < C; i += 4) {
+            *reinterpret_cast<float4*>(f + i) = *reinterpret_cast<const float4*>(red + n0 + i);
+            *reinterpret_cast<int4*>(at + i) = *reinterpret_cast<const int4*>(sRow + tb * N + n0 + i);
+          }
+          if (t >= D) continue;
+          if (item.z >= 0) {                         // rows that do not exist are not joined
+#pragma unroll
+            for (int i = 0; i < C; ++i) part[(n0 + i) * D] = __uint_as_float(o[i]) * f[i];
+          } else {
+#pragma unroll
+            for (int i = 0; i < C; ++i)
+              if (at[i] >= 0) out[(at[i] >> 8) * p.o_ld + (at[i] & 255) * D] = __float2bfloat16(__uint_as_float(o[i]) * f[i]);
+          }
+        }
+        tc_fence_before_sync();
+        few_any<128>(bar, false);                    // sums, maxima and the row tables have been read
+        if (lane == 0) mbar_arrive(&t_empty[tb]);
+      }
+      if (k >= mine) break;
       const uint32_t g = few_turn(k, grp, others), s = g % kStages, ph = k & 1u;
       const uint32_t tb = grp * 2 + (items & 1u);
       // a warp whose wait ran out (what it reads of the tile may then be anything) goes to the vote; the group leaves there together
@@ -679,7 +765,7 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
       ok = __all_sync(0xFFFFFFFFu, ok);                              // the aligned tcgen05 instructions need a converged warp
       float kf = p.scale_log2;
       int vbyte = 0;
-      bool high = first;
+      bool high = false;
       float sc[C];
       // scores of C rows from n0 on (log2 domain)
       auto scores = [&](int n0) {
@@ -717,107 +803,128 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
           if (S::kEarly && lane == 0) mbar_arrive(&empty[s]);
           high |= vbyte > top[7] + 3 && vbyte != 255;                // NaN needs no reference
         }
-#pragma unroll 1
-        for (int n0 = 0; n0 < R; n0 += C) {
-          scores(n0);
+        if constexpr (R == C) {
+          scores(0);
 #pragma unroll
           for (int i = 0; i < C; i += 4) {
-            const float4 m = *reinterpret_cast<const float4*>(m_mine + n0 + i);
+            const float4 m = *reinterpret_cast<const float4*>(m_mine + i);
             high |= !(sc[i] <= m.x + kCaRescale) || !(sc[i + 1] <= m.y + kCaRescale) || !(sc[i + 2] <= m.z + kCaRescale) ||
                     !(sc[i + 3] <= m.w + kCaRescale);
           }
         }
       }
-      tc_fence_before_sync();
-      // lazy: a reference maximum moves only when a score exceeds it by more than 2^8 (or is NaN)
-      const bool moves = few_any<128>(bar, high || !ok);
+      // Lazy: a reference maximum moves only when a score exceeds it by more than 2^8 (or is NaN).  Scores of a few rows stay in
+      // registers from one vote to the weights.  Those of many are read twice; there the weights are made at once, with the
+      // references as they are, which is nearly always right, and made again where the vote says that one has to move.
+      bool moves = first, out = false;
+      if constexpr (R == C) {
+        tc_fence_before_sync();
+        moves = few_any<128>(bar, high || first || !ok);
+      }
       // the product of the group's last tile has landed: its P buffer is free, its sums may be rescaled
       if (k > 0) ok = ok && few_wait(&pv_done[grp], ph ^ 1u, p.status);
       ok = __all_sync(0xFFFFFFFFu, ok);
-      if (moves) {
+      for (;;) {
+        if (moves) {
+          if (ok) {
+            tc_fence_after_sync();
+#pragma unroll 1
+            for (int n0 = 0; n0 < R; n0 += C) {
+              if (R > C) scores(n0);
+              const float v = few_across<C>(sc, lane, [](float x, float y) { return max_nan(x, y); });
+              if (my_turn) red[(warp & 3) * N + n0 + my_row] = v;
+            }
+            if (F8) {
+              const int v = __reduce_max_sync(0xFFFFFFFFu, vbyte == 255 ? 0 : vbyte);
+              if (lane == 0) top[warp & 3] = v;
+            }
+          }
+          ok = !few_any<128>(bar, !ok);
+          out = !ok;
+          if (out) break;
+          // a reference exponent that is passed by more than 3 moves as the maxima do
+          const int old_ref = !F8 ? 0 : first ? -1024 : top[7], most = F8 ? max(max(top[0], top[1]), max(top[2], top[3])) : 0;
+          const int ref = most > old_ref + 3 ? most : old_ref;
+          const float rescale = F8 ? ex2(static_cast<float>(old_ref - ref)) : 1.f;
+          if (t < R) {
+            const float now = max_nan(max_nan(red[t], red[N + t]), max_nan(red[2 * N + t], red[3 * N + t]));
+            const float old = first ? -1.0e29f : m_mine[t];
+            red[t] = !(now <= old + kCaRescale) ? now : old;
+          }
+          few_any<128>(bar, false);
+          if (!first) {
+            tc_fence_after_sync();
+#pragma unroll 1
+            for (int n0 = 0; n0 < R; n0 += 4) {
+              uint32_t o[4];
+              few_ld4(to + n0, o);
+              tc_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                o[i] = __float_as_uint(__uint_as_float(o[i]) * (ex2(m_mine[n0 + i] - red[n0 + i]) * rescale));
+              few_st4(to + n0, o);
+              tc_wait_st();
+            }
+            tc_fence_before_sync();
+            if (my_turn)
+              for (int n0 = my_row; n0 < R; n0 += C) sums[n0] *= ex2(m_mine[n0] - red[n0]);
+          }
+          few_any<128>(bar, false);                                  // everyone has read the old maxima
+          if (t < R) m_mine[t] = red[t];
+          if (F8 && t == 0) top[7] = ref;
+          few_any<128>(bar, false);
+        }
         if (ok) {
           tc_fence_after_sync();
+          // A key's weights are a row of P.  The sums take bf16 weights as rounded, as the tensor core multiplies them; fp16 ones, which
+          // hold the value's exponent as well, before they are rounded.
+          const float vf = vbyte == 255 ? __int_as_float(0x7FC00000) : ex2(static_cast<float>(vbyte - top[7] + 4));
 #pragma unroll 1
           for (int n0 = 0; n0 < R; n0 += C) {
             if (R > C) scores(n0);
-            const float v = few_across<C>(sc, lane, [](float x, float y) { return max_nan(x, y); });
-            if (my_turn) red[(warp & 3) * N + n0 + my_row] = v;
-          }
-          if (F8) {
-            const int v = __reduce_max_sync(0xFFFFFFFFu, vbyte == 255 ? 0 : vbyte);
-            if (lane == 0) top[warp & 3] = v;
-          }
-        }
-        ok = !few_any<128>(bar, !ok);
-        if (!ok) break;
-        // a reference exponent that is passed by more than 3 moves as the maxima do
-        const int old_ref = !F8 ? 0 : first ? -1024 : top[7], most = F8 ? max(max(top[0], top[1]), max(top[2], top[3])) : 0;
-        const int ref = most > old_ref + 3 ? most : old_ref;
-        const float rescale = F8 ? ex2(static_cast<float>(old_ref - ref)) : 1.f;
-        if (t < R) {
-          const float now = max_nan(max_nan(red[t], red[N + t]), max_nan(red[2 * N + t], red[3 * N + t]));
-          const float old = first ? -1.0e29f : m_mine[t];
-          red[t] = !(now <= old + kCaRescale) ? now : old;
-        }
-        few_any<128>(bar, false);
-        if (!first) {
-          tc_fence_after_sync();
-#pragma unroll 1
-          for (int n0 = 0; n0 < R; n0 += 4) {
-            uint32_t o[4];
-            few_ld4(to + n0, o);
-            tc_wait_ld();
+            uint32_t w[C / 2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              o[i] = __float_as_uint(__uint_as_float(o[i]) * (ex2(m_mine[n0 + i] - red[n0 + i]) * rescale));
-            few_st4(to + n0, o);
-            tc_wait_st();
-          }
-          tc_fence_before_sync();
-          if (my_turn)
-            for (int n0 = my_row; n0 < R; n0 += C) sums[n0] *= ex2(m_mine[n0] - red[n0]);
-        }
-        few_any<128>(bar, false);                                    // everyone has read the old maxima
-        if (t < R) m_mine[t] = red[t];
-        if (F8 && t == 0) top[7] = ref;
-        few_any<128>(bar, false);
-      }
-      if (ok) {
-        tc_fence_after_sync();
-        // A key's weights are a row of P.  The sums take bf16 weights as rounded, as the tensor core multiplies them; fp16 ones, which
-        // hold the value's exponent as well, before they are rounded.
-        const float vf = vbyte == 255 ? __int_as_float(0x7FC00000) : ex2(static_cast<float>(vbyte - top[7] + 4));
-#pragma unroll 1
-        for (int n0 = 0; n0 < R; n0 += C) {
-          if (R > C) scores(n0);
-          uint32_t w[C / 2];
+            for (int i = 0; i < C; i += 4) {
+              const float4 m = *reinterpret_cast<const float4*>(m_mine + n0 + i);
+              const float x[4] = {sc[i] - m.x, sc[i + 1] - m.y, sc[i + 2] - m.z, sc[i + 3] - m.w};
+              const float e[4] = {ex2(x[0]), ex2(x[1]), ex2(x[2]), ex2(x[3])};       // masked: 0
+              if (R > C) high |= !(x[0] <= kCaRescale) || !(x[1] <= kCaRescale) || !(x[2] <= kCaRescale) || !(x[3] <= kCaRescale);
 #pragma unroll
-          for (int i = 0; i < C; i += 4) {
-            const float4 m = *reinterpret_cast<const float4*>(m_mine + n0 + i);
-            const float e[4] = {ex2(sc[i] - m.x), ex2(sc[i + 1] - m.y), ex2(sc[i + 2] - m.z), ex2(sc[i + 3] - m.w)};     // masked: 0
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              if constexpr (F8) {
-                w[i / 2 + h] = few_pack_half(e[2 * h] * vf, e[2 * h + 1] * vf);
-                sc[i + 2 * h] = e[2 * h];
-                sc[i + 2 * h + 1] = e[2 * h + 1];
-              } else {
-                w[i / 2 + h] = pack_bf16(e[2 * h], e[2 * h + 1]);
-                sc[i + 2 * h] = __uint_as_float(w[i / 2 + h] << 16);
-                sc[i + 2 * h + 1] = __uint_as_float(w[i / 2 + h] & 0xFFFF0000u);
+              for (int h = 0; h < 2; ++h) {
+                if constexpr (F8) {
+                  w[i / 2 + h] = few_pack_half(e[2 * h] * vf, e[2 * h + 1] * vf);
+                  sc[i + 2 * h] = e[2 * h];
+                  sc[i + 2 * h + 1] = e[2 * h + 1];
+                } else {
+                  w[i / 2 + h] = pack_bf16(e[2 * h], e[2 * h + 1]);
+                  sc[i + 2 * h] = __uint_as_float(w[i / 2 + h] << 16);
+                  sc[i + 2 * h + 1] = __uint_as_float(w[i / 2 + h] & 0xFFFF0000u);
+                }
               }
             }
-          }
-          if constexpr (R == 4) {
-            *reinterpret_cast<uint2*>(sp + (few_place<kPRow>(t, 0) << 4)) = make_uint2(w[0], w[1]);
-          } else {
+            if constexpr (R == 4) {
+              *reinterpret_cast<uint2*>(sp + (few_place<kPRow>(t, 0) << 4)) = make_uint2(w[0], w[1]);
+            } else {
 #pragma unroll
-            for (int i = 0; i < C / 8; ++i)
-              *reinterpret_cast<uint4*>(sp + (few_place<kPRow>(t, n0 / 8 + i) << 4)) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+              for (int i = 0; i < C / 8; ++i)
+                *reinterpret_cast<uint4*>(sp + (few_place<kPRow>(t, n0 / 8 + i) << 4)) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+            }
+            const float v = few_across<C>(sc, lane, [](float x, float y) { return x + y; });
+            if (my_turn) {
+              if (R == C) sums[my_row] = first ? v : sums[my_row] + v;
+              else red[(warp & 3) * N + n0 + my_row] = v;
+            }
           }
-          const float v = few_across<C>(sc, lane, [](float x, float y) { return x + y; });
-          if (my_turn) sums[n0 + my_row] = first ? v : sums[n0 + my_row] + v;
         }
+        if (R == C || moves) break;
+        moves = few_any<128>(bar, high || !ok);
+        if (!moves) break;
+      }
+      if (out) break;                                // the group leaves, and with it the kernel
+      if (ok) {
+        // the sums of this tile, which the same lanes have written
+        if (R > C && my_turn)
+          for (int n0 = my_row; n0 < R; n0 += C) sums[n0] = first ? red[(warp & 3) * N + n0] : sums[n0] + red[(warp & 3) * N + n0];
         if (!F8 && !seen) {                          // values that no row sees are cleared (0 * NaN would be NaN)
 #pragma unroll
           for (int c = 0; c < D / 64; ++c)
@@ -832,39 +939,7 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
           mbar_arrive(&p_full[grp]);
         }
       }
-      if ((flags & kFewLast) == 0) continue;
-      // ---- the end of an item
-      ok = ok && few_wait(&pv_done[grp], ph, p.status);
-      ok = !few_any<128>(bar, !ok);                  // all sums are there
-      if (!ok) break;                                // a wait ran out (the status word says so): the outputs are not written
-      tc_fence_after_sync();
-      const int4 item = sItem[tb];                   // first row of q, key head, slot
-      ++items;
-      const float back = F8 ? few_power(max(top[7], 0)) * 0.0625f : 1.f;                 // 2^(Eref - 4)
-      const float* all = sSum + grp * 4 * N;
-#pragma unroll 1
-      for (int n0 = 0; n0 < R; n0 += 4) {
-        uint32_t o[4];
-        few_ld4(to + n0, o);
-        tc_wait_ld();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int row = n0 + i, at = sRow[tb * N + row];
-          if (at < 0) continue;
-          const float sum = (all[row] + all[N + row]) + (all[2 * N + row] + all[3 * N + row]), v = __uint_as_float(o[i]) * back;
-          if (item.z >= 0) {
-            const int64_t part = (static_cast<int64_t>(piece) * 2 + item.z) * R + row;
-            if (t < D) p.po[part * D + t] = v;
-            if (t == 0) *reinterpret_cast<float2*>(p.pml + part * 2) = make_float2(m_mine[row], sum);
-          } else if (t < D) {
-            p.o[(item.x + (at >> 8)) * p.o_ld + static_cast<int64_t>(item.y * p.group + (at & 255)) * D + t] =
-                __float2bfloat16(sum > 0.f ? v / sum : v * 0.f);
-          }
-        }
-      }
-      tc_fence_before_sync();
-      few_any<128>(bar, false);                      // sums, maxima and the row tables have been read
-      if (lane == 0) mbar_arrive(&t_empty[tb]);
+      pending = (flags & kFewLast) != 0;
     }
   }
 
@@ -883,22 +958,15 @@ __global__ void __launch_bounds__(128) cache_few_join_kernel(const CacheFewParam
   chain_next();
   chain_wait();
   const int b = blockIdx.y, kvh = blockIdx.x, row = blockIdx.z * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int all = fp.pre[p.batch] * p.hk, pieces = few_pieces(all, ctas);
-  const int tiles = fp.pre[b + 1] - fp.pre[b], from = fp.pre[b] * p.hk + kvh * tiles;
+  const int all = fp.pre[p.batch] * p.hk, tiles = fp.pre[b + 1] - fp.pre[b], from = fp.pre[b] * p.hk + kvh * tiles;
   if (tiles == 0) return;
-  // the piece of a place x is the last one whose cut is not behind it
-  auto piece = [&](int x) {
-    int c = static_cast<int>((static_cast<int64_t>(x) * pieces + pieces - 1) / all);
-    while (c > 0 && few_cut(all, c, pieces) > x) --c;
-    while (few_cut(all, c + 1, pieces) <= x) ++c;
-    return c;
-  };
-  const int c0 = piece(from), c1 = piece(from + tiles - 1);
+  const CacheFewCuts cuts(all, few_pieces(all, ctas));
+  const int c0 = cuts.piece(from), c1 = cuts.piece(from + tiles - 1);
   if (c0 == c1) return;
   int q_begin, q_len, k_len;
   ca_sequence(p, b, q_begin, q_len, k_len, false);
   if (row >= q_len * p.group) return;
-  const int first_slot = few_cut(all, c0, pieces) == from ? 0 : 1;
+  const int first_slot = cuts.cut(c0) == from ? 0 : 1;
   auto part = [&](int c) { return (c * 2 + (c == c0 ? first_slot : 0)) * R + row; };
   float m = -1.0e29f;
   for (int c = c0 + lane; c <= c1; c += 32) m = max_nan(m, p.pml[part(c) * 2]);
