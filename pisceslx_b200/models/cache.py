@@ -78,6 +78,9 @@ class YvPagedKVCache:
         if cfg.attention_window is not None and cfg.sliding_window is not None:
             raise ValueError("attention_window masks keys where they lie, sliding_window moves them: one of the two")
         self.fp8 = cfg.dtype == torch.float8_e4m3fn
+        if self.pages_only and not self.continues:
+            raise ValueError(f"8-bit pages, and windows, are for heads of 64 or 128 numbers and pages of a multiple of 16 tokens, bf16 or 8 "
+                             f"bits: heads of {head_dim}, pages of {cfg.block_size}, {cfg.dtype}")
         page = lambda: torch.zeros(shape, dtype=torch.uint8, device=device).view(cfg.dtype) if self.fp8 else \
             torch.zeros(shape, dtype=cfg.dtype, device=device)
         self.k = [page() for _ in range(n_layer)]
@@ -96,6 +99,12 @@ class YvPagedKVCache:
     def pages_only(self) -> bool:
         """Whether attention has to go through ``ops.cache`` (8-bit pages, or a window over them)."""
         return self.fp8 or self.cfg.attention_window is not None
+
+    @property
+    def continues(self) -> bool:
+        """Whether ``ops.cache`` reads these pages on their device, so that a prompt's later portion can attend to earlier ones."""
+        return torch.device(self.device).type != "cuda" or (self.d in (64, 128) and self.cfg.block_size % 16 == 0 and
+                                                            self.cfg.dtype in (torch.bfloat16, torch.float8_e4m3fn))
 
     def scales(self, idx: int) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
         """Exponent bytes of a layer's keys and values in 8 bits, else (None, None)."""
@@ -242,6 +251,10 @@ class YvPagedLayeredCache(YvPagedKVCache):
         self.layer_offset = 0
         self.reach = reach
 
+    @property
+    def continues(self) -> bool:
+        return True                                   # these layers read pages in ways of their own
+
     def rows(self, idx: int) -> torch.Tensor:
         if self.v[idx - self.layer_offset] is not None:
             raise TypeError("this layer stores keys and values: use layer()")
@@ -260,6 +273,9 @@ def cache_for_model(cfg, device: torch.device, num_blocks: int, block_size: Opti
                     n_layer: Optional[int] = None, dtype: torch.dtype = torch.bfloat16, attention_window: Optional[int] = None,
                     first_tokens: int = 0) -> YvPagedKVCache:
     """``dtype`` float8_e4m3fn, ``attention_window`` and ``first_tokens``: see ``YvCacheConfig``."""
+    if tp_size > 1 and attention_window is not None:
+        # there prompts are padded at their end, and a prompt's last row is taken for its last token
+        raise ValueError("attention_window: not with tensor parallelism")
     cc = YvCacheConfig(block_size=block_size or cfg.kv_cache_block_size, num_blocks=num_blocks, dtype=dtype,
                        attention_window=attention_window, first_tokens=first_tokens)
     if cfg.layer_specs:

@@ -161,6 +161,8 @@ def _prefill(model, ids: torch.Tensor, cache: YvPagedKVCache, seq_ids: List[int]
     trunk = model.model
     pad = (-S) % _tp_size(model)
     if pad:
+        if cache.cfg.attention_window is not None:
+            raise ValueError("attention_window: not with prompts that tensor parallelism pads")
         ids = torch.cat([ids, ids.new_zeros(B, pad)], dim=1)
     starts = [cache.lengths[s] for s in seq_ids]
     ctx = trunk.build_context(B, S + pad, ids.device)

@@ -19,7 +19,7 @@ from . import kernels, reference as ref, status_word
 def kv_cache_write_fp8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
                        v_scale: torch.Tensor, slot_map: torch.Tensor) -> None:
     """Append rows k/v [T, hk*d] (they may be column ranges of a projection) to the pages of codes and exponent bytes at flat slots
-    ``slot_map`` (int32, -1 = skip; of two rows for one slot either may stay)."""
+    ``slot_map`` (int32, -1 = skip; a slot has one row at most: of two, parts of both may stay)."""
     if k.is_cuda:
         kernels().kv_cache_write_fp8(k, v, k_cache, v_cache, k_scale, v_scale, slot_map, status_word(k.device))
         return
@@ -52,8 +52,8 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     behind a sequence's end does not matter.  A value that is NaN or infinite may reach all of its sequence's new tokens, those that
     it is hidden from among them; a key only those that see it.
 
-    Rows of ``q`` behind the last sequence: those of ``out`` are left as they are; without ``out`` they are zero.  ``splits``: key ranges
-    that are worked on at the same time (0: a rule on the sizes)."""
+    Rows of ``q`` behind the last sequence: those of ``out`` are left as they are; without ``out`` they are zero.  ``splits``: ranges
+    that the keys of a block of queries are cut in (0: a rule on the sizes); calls with few tokens cut them in a way of their own."""
     d = q.shape[-1]
     scale = d ** -0.5 if scale is None else scale
     if window is not None and window <= 0:

@@ -179,7 +179,7 @@ class YvInferenceEngine:
         if len(tokens) == 1 and self.cache.lengths[seq_id] > 0:
             logits = self.graph.step(list(tokens), [seq_id])
             return logits[[0] * len(want)] if want else None
-        size = self.cfg.prefill_portion if getattr(self.model, "supports_portions", False) else 0
+        size = self.cfg.prefill_portion if getattr(self.model, "supports_portions", False) and self.cache.continues else 0
         size = size or len(tokens)
         order = sorted(set(want))
         parts = []

@@ -119,6 +119,31 @@ def test_refusals(model):
     assert cache_for_model(model.cfg, dev, 2, dtype=F8).scales(0)[0].shape == (2, model.cfg.n_kv_head, model.cfg.kv_cache_block_size)
 
 
+def test_pages_that_the_gpu_cannot_read_are_not_continued():
+    """The kernels take heads of 64 or 128 numbers and pages of a multiple of 16 tokens: a prompt over other pages runs as a whole."""
+    def at(d, block, dtype=torch.bfloat16):
+        cache = YvPagedKVCache(1, 1, d, YvCacheConfig(num_blocks=2, block_size=block, dtype=dtype), torch.device("cpu"))
+        here = cache.continues
+        cache.device = torch.device("cuda")
+        return here, cache.continues
+    assert at(64, 16) == at(128, 64) == at(64, 48, F8) == (True, True)
+    assert at(32, 16) == at(64, 8) == at(64, 16, torch.float32) == (True, False)
+    cache = YvPagedLayeredCache([{"row": 24}], YvCacheConfig(num_blocks=2, block_size=8), torch.device("cpu"))
+    cache.device = torch.device("cuda")
+    assert cache.continues
+
+
+def test_a_window_is_refused_where_prompts_are_padded(model, monkeypatch):
+    with pytest.raises(ValueError, match="tensor parallelism"):
+        cache_for_model(model.cfg, torch.device("cpu"), 2, tp_size=2, attention_window=8)
+    from pisceslx_b200.models import generation
+    engine = _engine(model, attention_window=8)
+    engine.cache.add_sequence(1)
+    monkeypatch.setattr(generation, "_tp_size", lambda m: 2)
+    with pytest.raises(ValueError, match="pads"):
+        generation._prefill(model, torch.zeros(1, 3, dtype=torch.long), engine.cache, [1])
+
+
 def test_the_command_line_reaches_the_engine(monkeypatch):
     import sys
     import manage
