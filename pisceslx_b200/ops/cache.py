@@ -52,7 +52,7 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     behind a sequence's end does not matter.  A value that is NaN or infinite may reach all of its sequence's new tokens, those that
     it is hidden from among them; a key only those that see it.
 
-    Rows of ``q`` behind the last sequence: those of ``out`` are left as they are; without ``out`` they are zero.  ``splits``: ranges
+    Rows of ``q`` that belong to no sequence: those of ``out`` are left as they are; without ``out`` they are zero.  ``splits``: ranges
     that the keys of a block of queries are cut in (0: a rule on the sizes); calls with few tokens cut them in a way of their own."""
     d = q.shape[-1]
     scale = d ** -0.5 if scale is None else scale

@@ -241,7 +241,8 @@ int tile_splits(const CacheAttnArgs& a) {
   const CacheGrid g = cache_grid(a);
   const int sms = sm_count();
   int64_t keys = static_cast<int64_t>(a.table_width) * a.block;
-  if (a.window > 0) keys = keys < a.window + a.first + a.max_q ? keys : a.window + a.first + a.max_q;
+  const int64_t seen = static_cast<int64_t>(a.window) + a.first + a.max_q;
+  if (a.window > 0 && seen < keys) keys = seen;
   // steps of an item: key tiles of a block of two query tiles, pairs of key tiles of a lone one
   const double steps = static_cast<double>((keys + kCaTile - 1) / kCaTile) / (g.two ? 1 : 2);
   const int64_t room = (int64_t(256) << 20) / (a.total_q * a.hq * a.d * 4 + 1);              // ranges that the scratch has room for
@@ -298,7 +299,7 @@ CacheAttnParams cache_params(const CacheAttnArgs& a) {
   p.block = a.block; p.num_blocks = a.num_blocks; p.table_width = a.table_width;
   p.window = a.window; p.first = a.window > 0 ? a.first : 0;
   p.splits = a.splits;
-  p.zero_rest = a.zero_rest ? 1 : 0;
+  p.zero_rest = a.zero_rest;
   p.scale_log2 = a.scale * kLog2e;
   p.status = a.status;
   // rows of one copy: a power of two that divides a page
@@ -442,7 +443,7 @@ int launch_cache_attn(const CacheAttnArgs& a, cudaStream_t stream) {
     part.table += static_cast<int64_t>(b) * a.table_width;
     part.lens += b;
     if (a.cu_q != nullptr) part.cu_q += b;
-    part.zero_rest = a.zero_rest && b + part.batch == a.batch;
+    part.zero_rest = a.zero_rest & ((b + part.batch == a.batch ? 1 : 0) | (b == 0 ? 2 : 0));
     r = few != 0 ? launch_cache_few(part, few, b, stream) : launch_cache_tiles(part, b, stream);
   }
   return r;

@@ -72,6 +72,19 @@ __device__ __forceinline__ int64_t ca_item_of(int64_t r) {
   return r * gridDim.x + ((r & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
 }
 
+// Clears rows of o that belong to no sequence: behind the last one (zero_rest & 1), in front of the first (& 2).
+template <int D, int THREADS>
+__device__ __forceinline__ void ca_zero(const CacheAttnParams& p) {
+  if (p.zero_rest == 0) return;
+  const int64_t vecs = static_cast<int64_t>(p.hq) * D / 8, me = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x;
+  auto clear = [&](int64_t from, int64_t to) {
+    for (int64_t i = max(from, int64_t(0)) * vecs + me; i < min(to, p.total_q) * vecs; i += static_cast<int64_t>(gridDim.x) * THREADS)
+      *reinterpret_cast<uint4*>(p.o + i / vecs * p.o_ld + i % vecs * 8) = make_uint4(0, 0, 0, 0);
+  };
+  if ((p.zero_rest & 1) != 0) clear(p.cu_q != nullptr ? p.cu_q[p.batch] : p.first_row + p.batch, p.total_q);
+  if ((p.zero_rest & 2) != 0 && p.cu_q != nullptr) clear(0, p.cu_q[0]);
+}
+
 // The key tiles that a block of queries walks, as a list: those of the first tokens, then those from the window's first key on.
 struct CacheTiles {
   int lo, last, first_end;           // keys that any row of the block sees: [0, first_end) and [lo, last]
@@ -237,13 +250,7 @@ __global__ void __launch_bounds__(CacheAttn<D>::kThreads, 1) cache_attn_kernel(c
     tmem_alloc(tmem_slot, kTmemCols);
     tmem_relinquish();
   }
-  if (p.zero_rest != 0) {                              // rows that belong to no sequence
-    const int64_t used = p.cu_q != nullptr ? p.cu_q[p.batch] : p.first_row + p.batch;
-    const int64_t vecs = static_cast<int64_t>(p.hq) * D / 8;
-    for (int64_t i = (used < 0 ? 0 : used) * vecs + static_cast<int64_t>(blockIdx.x) * S::kThreads + threadIdx.x; i < p.total_q * vecs;
-         i += static_cast<int64_t>(gridDim.x) * S::kThreads)
-      *reinterpret_cast<uint4*>(p.o + i / vecs * p.o_ld + i % vecs * 8) = make_uint4(0, 0, 0, 0);
-  }
+  ca_zero<D, S::kThreads>(p);
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();

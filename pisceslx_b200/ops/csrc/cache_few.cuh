@@ -399,12 +399,7 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
   // the tensor memory is this kernel's before the next one may begin
   chain_next();
   chain_wait();
-  if (p.zero_rest != 0) {                                            // rows that belong to no sequence
-    const int64_t used = p.cu_q != nullptr ? p.cu_q[p.batch] : p.first_row + p.batch, vecs = static_cast<int64_t>(p.hq) * D / 8;
-    for (int64_t i = (used < 0 ? 0 : used) * vecs + static_cast<int64_t>(blockIdx.x) * S::kThreads + tid; i < p.total_q * vecs;
-         i += static_cast<int64_t>(gridDim.x) * S::kThreads)
-      *reinterpret_cast<uint4*>(p.o + i / vecs * p.o_ld + i % vecs * 8) = make_uint4(0, 0, 0, 0);
-  }
+  ca_zero<D, S::kThreads>(p);
   // Tiles in front of every sequence: each thread adds up a few sequences, the warps scan those sums, and the warps' are added.
   {
     const int each = (p.batch + S::kThreads - 1) / S::kThreads, b0 = min(tid * each, p.batch), b1 = min(b0 + each, p.batch);

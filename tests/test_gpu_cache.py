@@ -424,3 +424,49 @@ def test_nothing_to_do():
     pages = _empty(2, 16, 2, 64)
     C.kv_cache_write_fp8(*(torch.zeros(0, 128, dtype=torch.bfloat16, device=DEV),) * 2, *pages, none)
     assert C.kv_cache_read_fp8(*pages, none)[0].shape == (0, 128)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("new", [[3, 2], [70, 90]])
+def test_rows_in_front_of_the_first_sequence(fp8, new):
+    total = [400, 150]
+    case, dense = _case(new, total, 8, 2, 64, 64, fp8)
+    want, size = _oracle(case["q"], dense, new, total, None, 0, 64 ** -0.5)
+    case["q"] = torch.cat([torch.full_like(case["q"][:2], float("nan")), case["q"]])
+    case["cu"] += 2
+    torch.full((64, 8, 64), float("nan"), dtype=torch.bfloat16, device=DEV)                   # what the result may be given to lie in
+    got = _run(case, new)
+    check_status()
+    assert not got[:2].any()
+    _close(got[2:], want, size)
+    out = torch.full_like(case["q"], 3.0)
+    _run(case, new, out=out)
+    assert torch.equal(out[2:], got[2:]) and torch.equal(out[:2], torch.full_like(out[:2], 3.0))
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("hq,hk,cu", [(4, 2, True), (4, 2, False), (96, 1, False)])
+def test_more_sequences_than_one_launch_holds(fp8, hq, hk, cu):
+    """1300 sequences of 0 to 70 tokens, one new token each or (with cu_q) none to two; 96 query heads over one key head."""
+    n = 1300
+    g = torch.Generator().manual_seed(3)
+    new = torch.randint(0, 3, (n,), generator=g).tolist() if cu else [1] * n
+    total = [max(a, m) for a, m in zip(torch.randint(0, 71, (n,), generator=g).tolist(), new)] if cu else torch.randint(0, 71, (n,), generator=g).tolist()
+    case, dense = _case(new, total, hq, hk, 64, 16, fp8, dirty=False)
+    want, size = _oracle(case["q"], dense, new, total, None, 0, 64 ** -0.5)
+    if not cu:
+        case["cu"] = None
+    got = _run(case, new)
+    check_status()
+    _close(got, want, size)
+
+
+def test_queries_that_share_their_memory():
+    new, total = [5], [300]
+    case, dense = _case(new, total, 4, 2, 64, 64, False)
+    one = case["q"][:1].clone()
+    case["q"] = one.expand(5, 4, 64)
+    got = _run(case, new)
+    case["q"] = one.repeat(5, 1, 1)
+    assert torch.equal(got, _run(case, new))
+    check_status()
