@@ -154,7 +154,6 @@ int launch_cache_read_fp8(const CacheRowsArgs& a, cudaStream_t stream) {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kFewMost = 64;
 
 int sm_count() {
   static PerDeviceInt count;
@@ -204,10 +203,25 @@ int run_cache_attn(const CacheAttnParams& p, unsigned grid, cudaStream_t stream)
   return static_cast<int>(cudaGetLastError());
 }
 
-// Rows (token, head of a group) that the kernel for few tokens holds, 0 where cache_attn_kernel takes the call.
+// Key tiles that a block of queries can see at most.
+int64_t most_tiles(const CacheAttnArgs& a) {
+  int64_t keys = static_cast<int64_t>(a.table_width) * a.block;
+  const int64_t seen = static_cast<int64_t>(a.window) + a.first + a.max_q;
+  if (a.window > 0 && seen < keys) keys = seen;
+  return (keys + kCaTile - 1) / kCaTile;
+}
+
+// Rows (token, head of a group) that the kernel for few tokens holds, 0 where cache_attn_kernel takes the call.  That one would
+// have to widen 8-bit pages first: 16 sequences of 8192 tokens with 16 new ones, 4 heads a group: 115 us here, 17 new ones there 211.
+// Pages in bf16 it reads as they are, and its 128 rows cost no more than the keys' bytes.  It is the slower one where its key
+// ranges are uneven or too short, that is for up to 16 rows and many sequences (64 of up to 3000 tokens, 8 key heads, one new one:
+// 137 us against 121 here; 16 of 8192: 98 and 98) or for little in all (one of 2048 tokens: 16.4 and 13.8; of 8192: 29.6 and 28.7;
+// of 32768: 49 and 53).  More rows it takes always (16 of 8192 tokens with 8 new ones: 98 us, 131 here).
+constexpr int kFewMost = 64, kFewMostWide = 16;
 int few_rows(const CacheAttnArgs& a) {
-  const int64_t rows = static_cast<int64_t>(a.max_q) * (a.hq / a.hk);
-  if (rows > kFewMost) return 0;
+  const int64_t rows = static_cast<int64_t>(a.max_q) * (a.hq / a.hk), heads = static_cast<int64_t>(a.batch) * a.hk;
+  if (rows > (a.k_scale != nullptr ? kFewMost : kFewMostWide)) return 0;
+  if (a.k_scale == nullptr && heads < sm_count() && heads * most_tiles(a) > 4 * sm_count()) return 0;
   int r = 4;
   while (r < rows) r *= 2;
   return r;
@@ -240,11 +254,8 @@ namespace {
 int tile_splits(const CacheAttnArgs& a) {
   const CacheGrid g = cache_grid(a);
   const int sms = sm_count();
-  int64_t keys = static_cast<int64_t>(a.table_width) * a.block;
-  const int64_t seen = static_cast<int64_t>(a.window) + a.first + a.max_q;
-  if (a.window > 0 && seen < keys) keys = seen;
   // steps of an item: key tiles of a block of two query tiles, pairs of key tiles of a lone one
-  const double steps = static_cast<double>((keys + kCaTile - 1) / kCaTile) / (g.two ? 1 : 2);
+  const double steps = static_cast<double>(most_tiles(a)) / (g.two ? 1 : 2);
   const int64_t room = (int64_t(256) << 20) / (a.total_q * a.hq * a.d * 4 + 1);              // ranges that the scratch has room for
   const double sums = static_cast<double>(a.total_q) * a.hq * a.d * 8;                       // bytes written and read, per range
   int best = 1;
@@ -326,8 +337,12 @@ int run_cache_few(const CacheFewParams& p, int rows, unsigned grid, cudaStream_t
     case 4: return run_cache_few<D, F8, 4>(p, grid, stream);
     case 8: return run_cache_few<D, F8, 8>(p, grid, stream);
     case 16: return run_cache_few<D, F8, 16>(p, grid, stream);
-    case 32: return run_cache_few<D, F8, 32>(p, grid, stream);
-    default: return run_cache_few<D, F8, 64>(p, grid, stream);
+    case 32:
+      if constexpr (F8) return run_cache_few<D, F8, 32>(p, grid, stream);
+      return -9;
+    default:
+      if constexpr (F8) return run_cache_few<D, F8, 64>(p, grid, stream);
+      return -9;
   }
 }
 

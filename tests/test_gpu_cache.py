@@ -470,3 +470,16 @@ def test_queries_that_share_their_memory():
     case["q"] = one.repeat(5, 1, 1)
     assert torch.equal(got, _run(case, new))
     check_status()
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("window,first", [(None, 0), (5000, 200)])
+@pytest.mark.parametrize("new,total,cu", [([1], [20000], True), ([1, 1, 1], [9000, 0, 14001], False), ([4, 2], [4, 12345], True)])
+def test_few_tokens_of_long_sequences(new, total, cu, window, first, fp8):
+    case, dense = _case(new, total, 32, 8, 128, 64, fp8, window=window, first=first)
+    want, size = _oracle(case["q"], dense, new, total, window, first, 128 ** -0.5)
+    if not cu:
+        case["cu"] = None
+    got = _run(case, new, window=window, first_tokens=first)
+    check_status()
+    _close(got, want, size)
