@@ -199,8 +199,7 @@ int run_cache_attn(const CacheAttnParams& p, unsigned grid, cudaStream_t stream)
     if (e != cudaSuccess) return static_cast<int>(e);
     configured.cur() = 1;
   }
-  cache_attn_kernel<D><<<grid, S::kThreads, S::kTotal, stream>>>(p);
-  return static_cast<int>(cudaGetLastError());
+  return launch_chained(cache_attn_kernel<D>, dim3(grid), dim3(S::kThreads), S::kTotal, stream, 0, p);
 }
 
 // Key tiles that a block of queries can see at most.

@@ -250,10 +250,13 @@ __global__ void __launch_bounds__(CacheAttn<D>::kThreads, 1) cache_attn_kernel(c
     tmem_alloc(tmem_slot, kTmemCols);
     tmem_relinquish();
   }
-  ca_zero<D, S::kThreads>(p);
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
+  // the tensor memory is this kernel's before the next one may begin
+  chain_next();
+  chain_wait();
+  ca_zero<D, S::kThreads>(p);
   const uint32_t tmem_base = *tmem_slot;
 
   if (warp >= 8) regs_give<S::kOtherRegs>();
