@@ -700,13 +700,18 @@ __global__ void __launch_bounds__(128) cache_attn_merge_kernel(const CacheAttnPa
   float acc[E], l = 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll 4
   for (int s = 0; s < p.splits; ++s) {
     const float2 ml = *reinterpret_cast<const float2*>(p.pml + (s * step + row) * 2);
-    const float f = exp2f(ml.x - m);
-    l += ml.y * f;
+    const float f = ex2(ml.x - m);
     const float* src = p.po + (s * step + row) * D + lane * E;
+    l += ml.y * f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] += src[e] * f;
+    for (int e = 0; e < E; e += 2) {
+      const float2 v = *reinterpret_cast<const float2*>(src + e);
+      acc[e] += v.x * f;
+      acc[e + 1] += v.y * f;
+    }
   }
   const float inv = l > 0.f ? 1.f / l : 0.f;
   uint32_t* dst = reinterpret_cast<uint32_t*>(p.o + row / p.hq * p.o_ld + row % p.hq * D + lane * E);
