@@ -53,7 +53,7 @@ struct CacheAttnParams {
 };
 
 constexpr int kCaTile = 128;                    // rows of a query tile, keys of a key tile
-constexpr int kCaPoly = 4;                      // pairs of 16 whose 2^x is a polynomial
+constexpr int kCaPoly = 3;                      // pairs of 16 whose 2^x is a polynomial (2: 160 us, 4: 159, 6: 162 where 3 takes 157, 512 of 16384 tokens)
 constexpr float kCaMask = -1.0e30f;
 constexpr float kCaRescale = 8.0f;              // log2 units
 
