@@ -1,6 +1,7 @@
 // Attention of few new tokens over cached ones (sm_100a): decode steps, drafts, short turns.  The arithmetic is that of
 // cache_attn.cuh; the keys are the rows of the products here, so that a tile of 128 of them meets R = 4 to 64 (token, query head)
-// rows, N = max(R, 16) columns, instead of 128, and what bounds the kernel is the bytes of keys and values:
+// rows, N = max(R, 16) columns, instead of 128 (of bf16 pages up to 16 rows: see few_rows in cache.cu).  Few rows are bounded by the
+// bytes of keys and values; from some 16 rows on by the chain from a tile's scores to its product with the values:
 //
 //   S^T[128 keys, N]  = K[128 keys, D] Q[N, D]^T            (SS, K-major)
 //   O^T[D, N]        += V[128 keys, D]^T P[128 keys, N]     (SS; V as stored and P as a key's thread writes it are MN-major)
@@ -21,14 +22,21 @@
 //   0..3, 4..7  softmax of a piece: thread t owns key t of a tile (TMEM lane t of S^T) and output dimension t; a row's reference
 //               maximum is shared and moves in large steps, and the group meets at one vote a tile on whether it has to
 //   8           one lane issues the products: of a tile with the values, then the scores of the piece's next tile
-//   9           rows of the next items' queries
+//   9           rows of the next items' queries (and, of 8 bits and up to 16 rows, their codes)
 //   10, 11      TMA, a piece each: a stage holds a tile of keys and values (and, of 8-bit pages, their exponent bytes), and what the
 //               other warps have to know of it
 //   12..15      (8-bit pages) values to fp16
 // Only warps 9 to 11 walk the line, and all loops are short: 16 warps in six roles share an instruction cache.  With a walk of both
 // pieces in each of them a third of all stalls was for instructions and an 8-bit tile took 1.5 to 1.8 us; with one warp that
 // copied for both pieces, 1.2.  For the same reason 16 rows at a time go through a loop that is not unrolled: with all 64 of a tile
-// unrolled, in registers, what is done once an item cost more than its tiles (18 sequences of 2048 tokens, 16 new ones: 270 us).
+// unrolled, in registers, what is done once an item cost more than its tiles (18 sequences of 2048 tokens, 16 new ones: 270 us;
+// 16 of them take 59 in loops).
+//
+// 8-bit pages, 32 query heads over 8 of 128: 64 sequences of 2048 to 4096 tokens, a new one each, 89 us (4.7 TB/s of codes, 71 % of a
+// copy's rate; a tile takes an SM 0.85 us, its bytes 0.75); 8 of up to 8192 with 5 new ones 51 us (17.8 for the bytes; a tile 1.4 us,
+// 1.75 with 16 new ones).  Of each call 12 us or so are the beginning, the last parts and the join.  Scores of a piece's next tile
+// ahead of a product with the values, in a second buffer, made it slower (one new token 1.11 us a tile for 0.83, four 1.41 for
+// 1.04), and so did, from 32 rows on, loads of the next 16 rows' scores in front of the weights of these (2 to 5 %).
 #pragma once
 #include "cache_attn.cuh"
 #include "chain.cuh"
