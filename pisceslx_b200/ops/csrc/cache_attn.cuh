@@ -21,8 +21,9 @@
 // 32 query heads over 8 of 128: 512 tokens of 16384 157 us (863 TFLOP/s; 82 at the measured peak), 4096 of 32768 over 8-bit pages
 // 2022 us (1020 TFLOP/s; 1257).  A step, a key tile for both query tiles, takes 3700 cycles where its products take 2048: the
 // softmax of a half (2000) and the products of that half (1000, and as much behind the other's) follow one another, and both halves
-// with their scores, weights and sums fill the tensor memory, so that there is no room for a half's next scores.  Weights handed over
-// in two portions of 64 keys: 161 us.  An item costs 6 us to begin and to end besides.
+// with their scores, weights and sums fill the tensor memory, so that there is no room for a half's next scores.  In parts of 64 keys
+// there is, but their products read the query tile twice as often (180 us).  Weights handed over in two portions: 161 us.  An item
+// costs 6 us to begin and to end besides.
 //
 // What a page holds past the end of a sequence, or in front of everything that the block sees, may be anything: its scores are
 // masked and its values cleared (a zero weight times NaN is NaN).
