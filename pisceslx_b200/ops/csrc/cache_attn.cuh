@@ -60,7 +60,8 @@ struct CacheAttnParams {
 };
 
 constexpr int kCaTile = 128;                    // rows of a query tile, keys of a key tile
-constexpr int kCaPoly = 3;                      // pairs of 16 whose 2^x is a polynomial (2: 160 us, 4: 159, 6: 162 where 3 takes 157, 512 of 16384 tokens)
+// pairs of 16 whose 2^x is a polynomial (512 of 16384 tokens: 2 160 us, 3 157, 4 159, 6 162)
+constexpr int kCaPoly = 3;
 constexpr float kCaMask = -1.0e30f;
 constexpr float kCaRescale = 8.0f;              // log2 units
 

@@ -34,7 +34,7 @@ struct CacheAttnArgs {
   int window = 0, first = 0;                   // 0 = no window
   float scale = 1.f;
   int splits = 1;                              // key ranges of a query block, see cache_attn_plan
-  int zero_rest = 0;                           // rows of o that are cleared (else left alone): 1 behind the last sequence, 2 in front of the first
+  int zero_rest = 0;                           // rows of o that are cleared: 1 behind the last sequence, 2 in front of the first
   void* scratch = nullptr;                     // as many bytes as the plan says
   int wide_batch = 0;
   uint32_t* status = nullptr;
