@@ -12,7 +12,9 @@
 // and a row's are factors of the sums.  Value codes are widened to fp16, which holds them all, by four warps between the copy and
 // the product (one conversion for two codes; to bf16, with the exponent in it, took five operations and bounded the kernel); their
 // exponents go into the weights, fp16 too: w = p 2^(E - Eref + 4) with a reference Eref at least E - 3, at most 2^15.  fp16 keeps 11
-// bits of weights down to 2^-18 of the largest, and is off by 2^-29 of it below, where a row of bf16 weights keeps 8 bits.
+// bits of weights down to 2^-18 of the largest, and is off by 2^-29 of that below.  The largest may carry no weight for a row (its key is
+// hidden from it, or unlikely), so this is for value rows of about one size: once the exponents that an item has met are kFewSpread
+// apart, its tiles go as bf16, weights and values, with 8 bits of each weight as far as sums in 32 bits reach.
 //
 // The key tiles of all sequences and key heads form one line, which is cut into equal pieces, two for every SM: the kernel ends
 // everywhere at the same time whatever the lengths are, and nothing but the lengths on the device decides.  A (sequence, head) that
@@ -144,6 +146,12 @@ struct alignas(16) CacheFewTile {
   int key, flags, lo, last, first_end, pad[3];
   __device__ __forceinline__ bool seen(int k) const { return k <= last && (k >= lo || k < first_end); }
 };
+// Exponents of an item's seen values that fp16 weights hold: w = p 2^(E - Eref + 4) is off by 2^-25 where it is below 2^-14, and the
+// largest of a row is 2^(4 - kFewSpread) at least.  That is 2^-22 of it for each key, at worst as far as one bf16 weight for
+// 8192 keys that are all rounded alike.
+constexpr int kFewSpread = 7;
+// What bf16 values are held by: e4m3 codes keep their 3 bits of mantissa where they are in fp16, moved to bf16's place.
+constexpr int kFewWidePower = 112;
 enum : int {
   kFewGroup = 1,                     // the piece
   kFewFirst = 2, kFewLast = 4,       // of its item
@@ -245,6 +253,23 @@ __device__ __forceinline__ uint32_t few_pack_half(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// The fp16 numbers that e4m3 codes stand for to bf16 numbers 2^-kFewWidePower as large, exactly: a larger exponent field's bias.  (NaN
+// does not stay one; it is in rows whose weights are NaN.)
+__device__ __forceinline__ uint4 few_wide_values(uint4 v) {
+  auto one = [](uint32_t h) { return (h & 0x80008000u) | ((h >> 3) & 0x0FF00FF0u); };
+  return make_uint4(one(v.x), one(v.y), one(v.z), one(v.w));
+}
+
+// Values of a tile whose weights are bf16: widened to fp16 by other warps as ever, then changed in place by the 128 threads that made the
+// weights.  Not inlined: the softmax warps' loop with this inside it was 8 % slower where it is not wanted (64 sequences of
+// 3000 tokens 114 us for 106).  bf16 weights and values for every tile, without a reference exponent: 133.
+__device__ __noinline__ bool few_widen_tile(uint64_t* bar, uint32_t parity, uint32_t* status, uint4* v, int n) {
+  if (!few_wait_warp(bar, parity, status)) return false;
+#pragma unroll 1
+  for (int i = 0; i < n; i += kCaTile) v[i] = few_wide_values(v[i]);
+  return true;
+}
+
 // 2^(byte - 127); byte 255 gives NaN
 __device__ __forceinline__ float few_power(uint32_t byte) {
   return byte == 255u ? __int_as_float(0x7FC00000) : byte == 0u ? __int_as_float(0x00400000) : __int_as_float(static_cast<int>(byte) << 23);
@@ -324,8 +349,8 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
   constexpr uint32_t kSlab = kCaTile * 128;                          // 128 rows x 64 columns of bf16
   constexpr int kPRow = N * 2;                                       // bytes of a key's weights
   constexpr uint32_t kIdescS = F8 ? make_idesc_e4m3(128, 2 * N) : make_idesc_bf16(128, N, false, false);
-  // the format fields of fp16 are zero
-  constexpr uint32_t kIdescPV = make_idesc_bf16(128, N, true, true) & (F8 ? ~((1u << 7) | (1u << 10)) : ~0u);
+  constexpr uint32_t kIdescPV = make_idesc_bf16(128, N, true, true);
+  constexpr uint32_t kIdescHalf = kIdescPV & ~((1u << 7) | (1u << 10));          // the format fields of fp16 are zero
 
   extern __shared__ uint8_t cf_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(cf_raw) + 1023) & ~uintptr_t(1023));
@@ -352,7 +377,7 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(raw_empty + 1);
   uint8_t* sByte = reinterpret_cast<uint8_t*>(bars) + 256;                               // [kStages][2][128]
   CacheFewTile* sTile = reinterpret_cast<CacheFewTile*>(sByte + kStages * 2 * kCaTile);  // [kStages]
-  volatile int* sFirst = reinterpret_cast<int*>(bars) + 60;                              // [2] whether the weights are an item's first
+  volatile int* sKind = reinterpret_cast<int*>(bars) + 60;                               // [2] the weights are: 1 an item's first, 2 bf16
   int4* sItem = reinterpret_cast<int4*>(sTile + kStages);                                // [2][2] first row of q, key head, slot
   int* sHi = reinterpret_cast<int*>(sItem + 4);                    // [2][2][N] last visible key of a row, -1 = none
   int* sRow = sHi + 4 * N;                                                               // [2][2][N] token << 8 | head of the group
@@ -621,10 +646,11 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
           if (!few_wait(&p_full[i], k & 1u, p.status) || (F8 && !few_wait(&v_full[i], k & 1u, p.status))) break;
           tc_fence_after_sync();
           const uint32_t aV = F8 ? smem_u32(sWide + i * S::kWide) : smem_u32(stage_v(s)), aP = smem_u32(sP + i * S::kP);
-          const uint32_t more = sFirst[i] == 0 ? 1u : 0u;
+          const int kind = sKind[i];
+          const uint32_t more = (kind & 1) == 0 ? 1u : 0u, idesc = !F8 || (kind & 2) != 0 ? kIdescPV : kIdescHalf;
 #pragma unroll
           for (int kk = 0; kk < kCaTile / 16; ++kk)
-            tc_mma_f16_ss(tO + i * N, make_smem_desc(aV + kk * 2048, kSlab, 1024), few_desc<kPRow>(aP + kk * 16 * kPRow), kIdescPV,
+            tc_mma_f16_ss(tO + i * N, make_smem_desc(aV + kk * 2048, kSlab, 1024), few_desc<kPRow>(aP + kk * 16 * kPRow), idesc,
                           kk != 0 ? 1u : more);
           tc_commit(&pv_done[i]);
           if (!S::kEarly) tc_commit(&empty[s]);
@@ -685,7 +711,7 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tS = tmem_base + lane_off + grp * S::kSCols, to = tO + lane_off + grp * N;
     float *m_mine = sM + grp * N, *red = sRed + grp * 4 * N;
-    int* top = sTop + grp * 8;                                       // [0..3] of the warps, [7] the reference byte
+    int* top = sTop + grp * 8;                                       // exponent bytes: [0..3] of the warps, [6] least, [7] reference
     uint8_t* sp = sP + grp * S::kP + t * kPRow;
     uint32_t k = 0, items = 0;                                       // tiles and items so far
     bool ok = true;
@@ -804,7 +830,9 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
           vbyte = seen ? sByte[s * 2 * kCaTile + kCaTile + t] : 0;
           __syncwarp();
           if (S::kEarly && lane == 0) mbar_arrive(&empty[s]);
-          high |= vbyte > top[7] + 3 && vbyte != 255;                // NaN needs no reference
+          const int2 ends = *reinterpret_cast<const int2*>(top + 6);
+          // what is not seen has the byte 0, NaN (255) needs no reference
+          high |= (vbyte > ends.y + 3) & (vbyte != 255) | seen & (vbyte < ends.x);
         }
         if constexpr (R == C) {
           scores(0);
@@ -819,7 +847,7 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
       // Lazy: a reference maximum moves only when a score exceeds it by more than 2^8 (or is NaN).  Scores of a few rows stay in
       // registers from one vote to the weights.  Those of many are read twice; there the weights are made at once, with the
       // references as they are, which is nearly always right, and made again where the vote says that one has to move.
-      bool moves = first, out = false;
+      bool moves = first, out = false, wide = false;
       if constexpr (R == C) {
         tc_fence_before_sync();
         moves = few_any<128>(bar, high || first || !ok);
@@ -839,15 +867,23 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
             }
             if (F8) {
               const int v = __reduce_max_sync(0xFFFFFFFFu, vbyte == 255 ? 0 : vbyte);
-              if (lane == 0) top[warp & 3] = v;
+              const int u = __reduce_min_sync(0xFFFFFFFFu, seen ? vbyte : 255);
+              if (lane == 0) top[warp & 3] = v | u << 8;
             }
           }
           ok = !few_any<128>(bar, !ok);
           out = !ok;
           if (out) break;
-          // a reference exponent that is passed by more than 3 moves as the maxima do
-          const int old_ref = !F8 ? 0 : first ? -1024 : top[7], most = F8 ? max(max(top[0], top[1]), max(top[2], top[3])) : 0;
-          const int ref = most > old_ref + 3 ? most : old_ref;
+          // a reference exponent that is passed by more than 3 moves as the maxima do; the least one moves a step more than it has to
+          const int old_ref = !F8 ? 0 : first ? -1024 : top[7];
+          int ref = 0, least = 0;
+          if (F8) {
+            const int most = max(max(top[0] & 255, top[1] & 255), max(top[2] & 255, top[3] & 255));
+            ref = most > old_ref + 3 ? most : old_ref;
+            least = min(min(top[0], top[1]) >> 8, min(top[2], top[3]) >> 8) - 1;         // the upper bytes order the words
+            least = first ? least : min(least, top[6]);
+            if (ref - least > kFewSpread) least = -1024;             // far enough: nothing below moves it
+          }
           const float rescale = F8 ? ex2(static_cast<float>(old_ref - ref)) : 1.f;
           if (t < R) {
             const float now = max_nan(max_nan(red[t], red[N + t]), max_nan(red[2 * N + t], red[3 * N + t]));
@@ -874,14 +910,19 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
           }
           few_any<128>(bar, false);                                  // everyone has read the old maxima
           if (t < R) m_mine[t] = red[t];
-          if (F8 && t == 0) top[7] = ref;
+          if (F8 && t == 0) {
+            top[6] = least;
+            top[7] = ref;
+          }
           few_any<128>(bar, false);
         }
         if (ok) {
           tc_fence_after_sync();
           // A key's weights are a row of P.  The sums take bf16 weights as rounded, as the tensor core multiplies them; fp16 ones, which
           // hold the value's exponent as well, before they are rounded.
-          const float vf = vbyte == 255 ? __int_as_float(0x7FC00000) : ex2(static_cast<float>(vbyte - top[7] + 4));
+          const int2 ends = *reinterpret_cast<const int2*>(top + 6);
+          wide = F8 && ends.y - ends.x > kFewSpread;
+          const float vf = vbyte == 255 ? __int_as_float(0x7FC00000) : ex2(static_cast<float>(vbyte - ends.y + (wide ? 4 + kFewWidePower : 4)));
 #pragma unroll 1
           for (int n0 = 0; n0 < R; n0 += C) {
             if (R > C) scores(n0);
@@ -904,6 +945,10 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
                   sc[i + 2 * h + 1] = __uint_as_float(w[i / 2 + h] & 0xFFFF0000u);
                 }
               }
+            }
+            if (F8 && wide) {                        // again, as bf16: a branch that is rarely taken costs less than two forms of each weight
+#pragma unroll
+              for (int i = 0; i < C; i += 2) w[i / 2] = pack_bf16(sc[i] * vf, sc[i + 1] * vf);
             }
             if constexpr (R == 4) {
               *reinterpret_cast<uint2*>(sp + (few_place<kPRow>(t, 0) << 4)) = make_uint2(w[0], w[1]);
@@ -934,11 +979,15 @@ __global__ void __launch_bounds__(CacheFew<D, F8, R>::kThreads, 1) cache_few_ker
 #pragma unroll
             for (int i = 0; i < 8; ++i) reinterpret_cast<uint4*>(stage_v(s) + c * kSlab + t * 128)[i] = make_uint4(0, 0, 0, 0);
         }
+        if (F8 && wide)
+          ok = few_widen_tile(&v_full[grp], ph, p.status, reinterpret_cast<uint4*>(sWide + grp * S::kWide) + t, S::kWide / 16);
+      }
+      if (ok) {
         fence_proxy_async_smem();
         tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) {
-          if ((warp & 3) == 0) sFirst[grp] = first ? 1 : 0;
+          if ((warp & 3) == 0) sKind[grp] = (first ? 1 : 0) | (wide ? 2 : 0);
           mbar_arrive(&p_full[grp]);
         }
       }
