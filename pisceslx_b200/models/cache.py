@@ -78,6 +78,8 @@ class YvPagedKVCache:
         if cfg.attention_window is not None and cfg.sliding_window is not None:
             raise ValueError("attention_window masks keys where they lie, sliding_window moves them: one of the two")
         self.fp8 = cfg.dtype == torch.float8_e4m3fn
+        if self.fp8 and cfg.sliding_window is not None:
+            raise ValueError("8-bit pages are read through whole tables, which sliding_window cuts: attention_window masks keys instead")
         if self.pages_only and not self.continues:
             raise ValueError(f"8-bit pages, and windows, are for heads of 64 or 128 numbers and pages of a multiple of 16 tokens, bf16 or 8 "
                              f"bits: heads of {head_dim}, pages of {cfg.block_size}, {cfg.dtype}")
@@ -102,9 +104,10 @@ class YvPagedKVCache:
 
     @property
     def continues(self) -> bool:
-        """Whether ``ops.cache`` reads these pages on their device, so that a prompt's later portion can attend to earlier ones."""
-        return torch.device(self.device).type != "cuda" or (self.d in (64, 128) and self.cfg.block_size % 16 == 0 and
-                                                            self.cfg.dtype in (torch.bfloat16, torch.float8_e4m3fn))
+        """Whether ``ops.cache`` reads these pages on their device, so that a prompt's later portion can attend to earlier ones.  Tables
+        that ``sliding_window`` cuts do not say where they begin."""
+        return self.cfg.sliding_window is None and (torch.device(self.device).type != "cuda" or (
+            self.d in (64, 128) and self.cfg.block_size % 16 == 0 and self.cfg.dtype in (torch.bfloat16, torch.float8_e4m3fn)))
 
     def scales(self, idx: int) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
         """Exponent bytes of a layer's keys and values in 8 bits, else (None, None)."""

@@ -169,6 +169,8 @@ def _prefill(model, ids: torch.Tensor, cache: YvPagedKVCache, seq_ids: List[int]
     if any(starts):
         if not getattr(model, "supports_portions", False):
             raise ValueError("this model's attention does not continue a prompt from the cache")
+        if not cache.continues:
+            raise ValueError("attention does not continue a prompt from these pages (see YvPagedKVCache.continues)")
         ctx.starts, ctx.lens = starts, [S] * B
         ctx.slots_of = lambda b, lo, hi: cache.slots(seq_ids[b], lo, hi)
         first = to_device(starts, torch.int32, ids.device)

@@ -1,0 +1,65 @@
+"""Which prompts may be continued from a cache: what is refused is refused before the sequence has grown."""
+import pytest
+import torch
+
+from pisceslx_b200 import YvConfig
+from pisceslx_b200.models import build_model, generation
+from pisceslx_b200.models.cache import YvCacheConfig, YvPagedKVCache
+from pisceslx_b200.serve.engine import YvEngineConfig, YvInferenceEngine
+
+TOKENS = torch.randint(0, 300, (80,), generator=torch.Generator().manual_seed(5)).tolist()
+
+
+def _model(**kw):
+    cfg = YvConfig.tiny_text_moe(vocab_size=300)
+    cfg.n_layer = 2
+    for k, v in kw.items():
+        setattr(cfg, k, v)
+    return build_model(cfg, "cpu", torch.float32, seed=1).eval()
+
+
+@pytest.fixture(scope="module")
+def model():
+    return _model()
+
+
+def _cache(model, **kw):
+    cfg = model.cfg
+    return YvPagedKVCache(cfg.n_layer, cfg.n_kv_head, cfg.head_dim, YvCacheConfig(block_size=16, num_blocks=16, dtype=torch.float32, **kw), torch.device("cpu"))
+
+
+def _run(model, cache, tokens):
+    return generation._prefill(model, torch.tensor([tokens]), cache, [1])
+
+
+def test_tables_that_are_cut_are_not_continued(model):
+    """A sliding window's tables hold a sequence's last pages only: a later portion would read others' tokens at other positions."""
+    cache = _cache(model, sliding_window=32)
+    assert not cache.continues and _cache(model).continues
+    cache.add_sequence(1)
+    _run(model, cache, TOKENS[:70])
+    before = (cache.lengths[1], list(cache.tables[1]), cache.alloc.available())
+    with pytest.raises(ValueError, match="continue"):
+        _run(model, cache, TOKENS[70:76])
+    assert before == (cache.lengths[1], list(cache.tables[1]), cache.alloc.available())
+
+
+def test_8_bit_pages_are_not_read_through_cut_tables():
+    with pytest.raises(ValueError, match="sliding_window"):
+        YvPagedKVCache(1, 1, 64, YvCacheConfig(num_blocks=2, dtype=torch.float8_e4m3fn, sliding_window=64), torch.device("cpu"))
+
+
+def test_pages_that_no_kernel_reads_are_refused_before_slots_are_taken(model, monkeypatch):
+    cache = _cache(model)
+    cache.add_sequence(1)
+    _run(model, cache, TOKENS[:20])
+    monkeypatch.setattr(YvPagedKVCache, "continues", property(lambda self: False))
+    with pytest.raises(ValueError, match="continue"):
+        _run(model, cache, TOKENS[20:50])
+    assert cache.lengths[1] == 20 and len(cache.tables[1]) == 2
+    fresh = _cache(model)
+    fresh.add_sequence(1)
+    assert _run(model, fresh, TOKENS[:50]).shape == (1, 300)                     # prompts from their start need no pages
+    engine = YvInferenceEngine(model, cfg=YvEngineConfig(num_blocks=16, block_size=16, prefill_portion=8, eos_token_id=-1))
+    engine.cache.add_sequence(1)
+    assert engine.run_tokens(1, TOKENS[:50], [49]).shape == (1, 300)             # as a whole
