@@ -206,10 +206,13 @@ class YvModelForCausalLM(nn.Module):
     @property
     def supports_portions(self) -> bool:
         """Whether a prompt may be continued from the cache at any position: all that a token sees of earlier ones is in the
-        cached keys and values (a state-space branch and the knowledge field look at the prompt as a whole), on one rank."""
+        cached keys and values (a state-space branch, the knowledge field and experts with a capacity look at the prompt as a
+        whole, a route that is kept from call to call is for the rows of one), on one rank."""
+        alone = lambda router: not router.drop_tokens and getattr(router, "path_stage_size", 1) == 1
         par, trunk = self.parallel, self.model
         return (par is None or (par.tp_size == 1 and getattr(par, "cp_size", 1) == 1)) and trunk.subconscious is None and \
-            all(type(blk) is YvTransformerBlock and type(blk.attention) is YvAttention and blk.ssm is None for blk in trunk.layers)
+            all(type(blk) is YvTransformerBlock and type(blk.attention) is YvAttention and blk.ssm is None and
+                (not blk.is_moe or alone(blk.mlp.router)) for blk in trunk.layers)
 
     def __init__(self, cfg: YvConfig, parallel=None):
         super().__init__()

@@ -63,3 +63,27 @@ def test_pages_that_no_kernel_reads_are_refused_before_slots_are_taken(model, mo
     engine = YvInferenceEngine(model, cfg=YvEngineConfig(num_blocks=16, block_size=16, prefill_portion=8, eos_token_id=-1))
     engine.cache.add_sequence(1)
     assert engine.run_tokens(1, TOKENS[:50], [49]).shape == (1, 300)             # as a whole
+
+
+def test_experts_with_a_capacity_see_prompts_as_a_whole():
+    """Which assignments a full expert drops depends on all tokens of the call."""
+    dropping = _model(moe_drop_tokens=True, moe_capacity_factor=0.5, moe_min_capacity=1)
+    assert any(blk.is_moe for blk in dropping.model.layers) and not dropping.supports_portions
+    kw = dict(num_blocks=16, block_size=16, eos_token_id=-1)
+    logits = []
+    for portion in (0, 9):
+        engine = YvInferenceEngine(dropping, cfg=YvEngineConfig(prefill_portion=portion, **kw))
+        engine.cache.add_sequence(1)
+        logits.append(engine.run_tokens(1, TOKENS, [79]))
+    assert torch.equal(*logits)
+    engine.cache.add_sequence(2)
+    engine.run_tokens(2, TOKENS[:40], [])
+    with pytest.raises(ValueError, match="continue"):
+        engine.run_tokens(2, TOKENS[40:50], [9])
+    assert engine.cache.lengths[2] == 40
+
+
+def test_routes_that_are_kept_from_call_to_call_are_not_those_of_another_portion():
+    model = _model(moe_gate_type="research", extra={"path_moe_stage_size": 2})
+    assert model.model.layers[-1].mlp.router.path_stage_size == 2 and not model.supports_portions
+    assert _model(moe_gate_type="research").supports_portions
