@@ -50,7 +50,9 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     Pages [blocks, block, hk, d] are bf16, or e4m3 codes with ``k_scale`` and ``v_scale`` as ``kv_cache_write_fp8`` leaves them; a page
     holds a multiple of 16 tokens, heads 64 or 128 numbers, and up to 128 query heads share a key head.  What a page holds
     behind a sequence's end does not matter.  8-bit values of one sequence may differ by up to 2^100 in size: beside larger ones, smaller
-    ones may count as zero for few tokens.  A value that is NaN or infinite may reach all of its sequence's new tokens, those that
+    ones may count as zero for few tokens.  More than 64 (token, query head of a key head) rows a sequence take scratch of 4 hk d bytes for
+    each 8-bit token that the table has room for, or that ``window`` and ``first_tokens`` let the new tokens see: a gigabyte at a time,
+    one sequence at least.  A value that is NaN or infinite may reach all of its sequence's new tokens, those that
     it is hidden from among them; a key only those that see it.
 
     Rows of ``q`` that belong to no sequence: those of ``out`` are left as they are; without ``out`` they are zero.  ``splits``: ranges

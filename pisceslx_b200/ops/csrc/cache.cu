@@ -210,6 +210,16 @@ int64_t most_tiles(const CacheAttnArgs& a) {
   return (keys + kCaTile - 1) / kCaTile;
 }
 
+// Rows that 8-bit keys of a sequence take once they are widened: as many as its table has room for, or as the new tokens' window and
+// the first tokens can see, in whole tiles (see CacheRoom; 512 new tokens with a window of 4096 over a table of 131072 tokens
+// of 8 heads of 128: 19 MB for 537).
+int widened_room(const CacheAttnArgs& a) {
+  const int64_t all = static_cast<int64_t>(a.table_width) * a.block;
+  if (a.window <= 0) return static_cast<int>(all);
+  const int64_t tiles = (static_cast<int64_t>(a.first) + kCaTile - 1) / kCaTile + (static_cast<int64_t>(a.window) + a.max_q - 2) / kCaTile + 2;
+  return static_cast<int>(tiles * kCaTile < all ? tiles * kCaTile : all);
+}
+
 // Rows (token, head of a group) that the kernel for few tokens holds, 0 where cache_attn_kernel takes the call.  That one would
 // have to widen 8-bit pages first: 16 sequences of 8192 tokens with 16 new ones, 4 heads a group: 115 us here, 17 new ones there 211.
 // Pages in bf16 it reads as they are, and its 128 rows cost no more than the keys' bytes.  It is the slower one where its key
@@ -284,7 +294,7 @@ int64_t cache_attn_plan(CacheAttnArgs& a) {
   int64_t bytes = part_bytes(a, 0);
   if (a.k_scale != nullptr) {
     // about a gigabyte at a time, one sequence at least
-    const int64_t one = static_cast<int64_t>(a.table_width) * a.block * a.hk * a.d * 4, fit = (int64_t(1) << 30) / one;
+    const int64_t one = static_cast<int64_t>(widened_room(a)) * a.hk * a.d * 4, fit = (int64_t(1) << 30) / one;
     a.wide_batch = static_cast<int>(fit < 1 ? 1 : fit < a.batch ? fit : a.batch);
     bytes += one * a.wide_batch;
   }
@@ -407,7 +417,7 @@ int launch_cache_tiles(const CacheAttnArgs& a, int first_row, cudaStream_t strea
                        static_cast<uint32_t>(p.group), static_cast<uint32_t>(p.per_tile));
   if (r != 0) return -10 + r;
   const bool wide = a.k_scale != nullptr;
-  p.room = a.table_width * a.block;
+  p.room = widened_room(a);
   const int64_t slots = wide ? static_cast<int64_t>(a.batch) * p.room : static_cast<int64_t>(a.num_blocks) * a.block;
   if (slots >= (1ll << 31)) return -3;
   if (wide) {
@@ -426,7 +436,7 @@ int launch_cache_tiles(const CacheAttnArgs& a, int first_row, cudaStream_t strea
   p.pml = p.po + (a.splits > 1 ? a.total_q * a.hq * a.splits * a.d : 0);
   if (wide) {
     CacheWidenArgs w = {a.k, a.v, a.k_scale, a.v_scale, wide_k, wide_v, a.table, a.lens, a.cu_q, a.table_width, a.block,
-                        a.num_blocks, a.hk, p.room, p.window, p.first, a.status};
+                        a.num_blocks, a.hk, p.room, a.max_q, p.window, p.first, a.status};
     const int64_t blocks = (static_cast<int64_t>(p.room) * 2 * a.hk * (a.d / 16) + 255) / 256;
     if (blocks > 0x7FFFFFFFll || a.batch > 65535) return -7;
     const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(a.batch));

@@ -41,7 +41,7 @@ struct CacheWidenArgs {
   const void *k, *v, *k_scale, *v_scale;
   void *ko, *vo;
   const int *table, *lens, *cu_q;
-  int table_width, block, num_blocks, hk, room, window, first;
+  int table_width, block, num_blocks, hk, room, max_q, window, first;
   uint32_t* status;
 };
 
@@ -51,7 +51,7 @@ struct CacheAttnParams {
   __nv_bfloat16* o;
   int64_t o_ld;
   float *po, *pml;
-  const int *cu_q, *table, *lens;   // without a table key j of sequence b has the slot b * room + j
+  const int *cu_q, *table, *lens;   // without a table key j of sequence b has the slot b * room + CacheRoom::row(j)
   int64_t total_q, items;
   int hq, hk, group, per_tile, batch, max_q, block, box, num_blocks, table_width;
   int window, first, two, splits, zero_rest, first_row, room;
@@ -128,6 +128,20 @@ struct CacheTiles {
   }
 };
 
+// Rows that the keys which a sequence's new tokens see have among the `room` of it that are widened: those of the first tokens' tiles,
+// then those from the window's first tile on (of CacheTiles the list for all new tokens, in whole tiles; a block's list is a part of it).
+struct CacheRoom {
+  int keep, skip;                    // keys below keep have rows of their own number, others lie skip rows further in front
+  __device__ __forceinline__ CacheRoom(int from, int window, int first) {
+    CacheTiles t;
+    t.set(from, from, window, first, 0, 1);
+    keep = t.ns * kCaTile;
+    skip = (t.w0 - t.ns) * kCaTile;
+  }
+  __device__ __forceinline__ int row(int key) const { return key < keep ? key : key - skip; }
+  __device__ __forceinline__ int key(int row) const { return row < keep ? row : row + skip; }
+};
+
 // Rows of q and cached tokens of sequence b; what is out of range is reported (if `report`) and counts as empty.
 __device__ __forceinline__ void ca_sequence(const CacheAttnParams& p, int b, int& q_begin, int& q_len, int& k_len, bool report) {
   q_begin = p.cu_q != nullptr ? p.cu_q[b] : p.first_row + b;
@@ -188,7 +202,6 @@ struct CacheItem : CacheTiles {
 
 // Flat slot of a key of sequence b; at a table entry outside the pool (reported) some valid one.
 __device__ __forceinline__ int ca_slot(const CacheAttnParams& p, int b, int key) {
-  if (p.table == nullptr) return b * p.room + key;
   const int bi = key / p.block;
   int page = p.table[static_cast<int64_t>(b) * p.table_width + bi];
   if (page < 0 || page >= p.num_blocks) {
@@ -290,7 +303,8 @@ __global__ void __launch_bounds__(CacheAttn<D>::kThreads, 1) cache_attn_kernel(c
         const int j = j0 + lane / boxes;
         if (j >= n) return -1;
         const int a = it.first_key(j) + (lane % boxes) * p.box;
-        return it.any(a, p.box) ? ca_slot(p, it.b, a) : -1;
+        if (!it.any(a, p.box)) return -1;
+        return p.table != nullptr ? ca_slot(p, it.b, a) : it.b * p.room + CacheRoom(it.shift, p.window, p.first).row(a);
       };
       int rows = look(0), next = -1;
       for (int t = 0; t < 2 && ok; ++t) {
@@ -659,19 +673,20 @@ __device__ __forceinline__ void ca_values(uint4 c, uint32_t most, uint32_t byte,
   hi = make_uint4(r[4], r[5], r[6], r[7]);
 }
 
-// Keys and values that the new tokens of a sequence see, from 8-bit pages to bf16 rows [sequence, room, hk, D] (what they do not
-// see is left alone).  A group of D / 16 lanes per row.  Bound by bytes: 3 for each number.
+// Keys and values that the new tokens of a sequence see, from 8-bit pages to bf16 rows [sequence, room, hk, D], see CacheRoom (what
+// they do not see is left alone).  A group of D / 16 lanes per row.  Bound by bytes: 3 for each number.
 template <int D>
 __global__ void __launch_bounds__(256) cache_widen_kernel(const CacheWidenArgs a) {
   constexpr int kLanes = D / 16;
   const int64_t at = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / kLanes;
   const int lane = threadIdx.x % kLanes, b = blockIdx.y;
-  const int key = static_cast<int>(at / (2 * a.hk));
-  int r = static_cast<int>(at - static_cast<int64_t>(key) * 2 * a.hk);
-  const int n = a.lens[b];
-  if (key >= n || n > a.room) return;                          // a length past the table: reported by the attention kernel
-  const int new_tokens = a.cu_q != nullptr ? a.cu_q[b + 1] - a.cu_q[b] : 1;
-  if (a.window > 0 && key <= n - new_tokens - a.window && key >= a.first) return;
+  const int row = static_cast<int>(at / (2 * a.hk));
+  int r = static_cast<int>(at - static_cast<int64_t>(row) * 2 * a.hk);
+  const int n = a.lens[b], new_tokens = a.cu_q != nullptr ? a.cu_q[b + 1] - a.cu_q[b] : 1;
+  // what is out of range is reported by the attention kernel, and read by nobody
+  if (row >= a.room || row >= n || static_cast<int64_t>(n) > static_cast<int64_t>(a.table_width) * a.block || new_tokens < 0 || new_tokens > a.max_q) return;
+  const int from = n - new_tokens, key = CacheRoom(from, a.window, a.first).key(row);
+  if (key >= n || (a.window > 0 && key <= from - a.window && key >= a.first)) return;
   const bool val = r >= a.hk;
   if (val) r -= a.hk;
   const int bi = key / a.block, off = key - bi * a.block;
@@ -686,7 +701,7 @@ __global__ void __launch_bounds__(256) cache_widen_kernel(const CacheWidenArgs a
   uint4 lo, hi;
   ca_values(c, byte, byte, lo, hi);
   uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(val ? a.vo : a.ko) +
-                                        ((static_cast<int64_t>(b) * a.room + key) * a.hk + r) * D) + 2 * lane;
+                                        ((static_cast<int64_t>(b) * a.room + row) * a.hk + r) * D) + 2 * lane;
   dst[0] = lo;
   dst[1] = hi;
 }

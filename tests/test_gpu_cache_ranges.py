@@ -1,4 +1,5 @@
-"""Attention of few tokens over 8-bit pages whose value rows differ much in size, against plain math in 64 bits."""
+"""Attention over 8-bit pages where sizes are unusual: value rows that differ much, tables far wider than what is seen, entries and lengths
+that are out of range.  Against plain math in 64 bits."""
 import pytest
 import torch
 
@@ -136,3 +137,44 @@ def test_the_number_of_rows_does_not_change_what_a_token_gets():
     want, size = _oracle(q, dense, [17], None, 0)
     _close(all_rows, want, size)
     _close(few, want[1:], size[1:])
+
+
+def _wide_table(args, width):
+    """The same call with a table of as many entries as a long stream has: those in front were given back, those behind are not used."""
+    table = torch.full((args[3].shape[0], width), -1, dtype=torch.int32, device=DEV)
+    table[:, :args[3].shape[1]] = args[3]
+    return args[:3] + (table,) + args[4:]
+
+
+@pytest.mark.parametrize("window,first", [(100, 0), (300, 4), (700, 200), (129, 128), (1, 0), (2000, 700)])
+def test_scratch_of_a_windowed_portion_follows_the_window(window, first):
+    news, total = [90, 33], [1900, 640]
+    args, scales, dense = _case("even", news, total, 8, 2, 128, 64, seed=window)
+    want, size = _oracle(args[0], dense, news, window, first)
+    _close(C.cache_attention(*args, window=window, first_tokens=first, **scales), want, size)
+    args = _wide_table(args, 40000)                                              # 2560000 tokens: 2.6 GB a sequence in bf16
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = C.cache_attention(*args, window=window, first_tokens=first, **scales)
+    check_status()
+    _close(got, want, size)
+    rows = -(-first // 128) * 128 + window + 90 + 256
+    # keys and values of what can be seen, and up to 32 ranges of sums in 32 bits
+    assert torch.cuda.max_memory_allocated() - before < 2 * (rows * 2 * 128 * 4) + 32 * 123 * 8 * 130 * 4 + (1 << 20)
+
+
+def test_widened_pages_of_a_batch_in_turns():
+    """Tables of 131072 tokens: two sequences of 8 heads of 128 are widened at a time."""
+    news, total = [40, 20, 33, 1, 17], [700, 300, 33, 260, 129]
+    args, scales, dense = _case("even", news, total, 32, 8, 128, 64)
+    want, size = _oracle(args[0], dense, news, None, 0)
+    _close(C.cache_attention(*args, **scales), want, size)
+    wide = _wide_table(args, 2048)
+    got = C.cache_attention(*wide, **scales)
+    check_status()
+    _close(got, want, size)
+    out = torch.full_like(args[0], 3.0)
+    C.cache_attention(*wide, out=out, splits=2, **scales)
+    check_status()
+    _close(out, want, size)
