@@ -147,7 +147,7 @@ __device__ __forceinline__ void ca_sequence(const CacheAttnParams& p, int b, int
   q_begin = p.cu_q != nullptr ? p.cu_q[b] : p.first_row + b;
   const int q_end = p.cu_q != nullptr ? p.cu_q[b + 1] : q_begin + 1;
   q_len = q_end - q_begin;
-  if (q_begin < 0 || q_end > p.total_q || q_len > p.max_q) {
+  if (q_begin < 0 || q_end > p.total_q || q_len < 0 || q_len > p.max_q) {
     if (report && p.status != nullptr) atomicOr(p.status, kStatusBadArgument);
     q_len = 0;
   }

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from pisceslx_b200.ops import cache as C
-from pisceslx_b200.ops import check_status
+from pisceslx_b200.ops import KernelStatusError, check_status
 from pisceslx_b200.ops import reference as ref
 
 pytestmark = pytest.mark.gpu
@@ -178,3 +178,36 @@ def test_widened_pages_of_a_batch_in_turns():
     C.cache_attention(*wide, out=out, splits=2, **scales)
     check_status()
     _close(out, want, size)
+
+
+@pytest.mark.parametrize("bad", ["table", "length", "negative", "queries", "backwards"])
+@pytest.mark.parametrize("new", [[2, 1], [16, 1], [90, 2]])
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("window", [None, 150])
+def test_what_is_out_of_range_is_reported_and_disturbs_no_other_sequence(bad, new, fp8, window):
+    """Bad entries in the middle of three sequences, in each of the kernels."""
+    news, total = [new[0], new[0], new[1]], [300, 200, 130]
+    (q, k, v, table, lens, cu, max_q), scales, dense = _case("even", news, total, 8, 2, 64, 64)
+    want, size = _oracle(q, dense, news, window, 0)
+    if not fp8:
+        k, v = (torch.ldexp(x.float(), (s.transpose(1, 2).int() - 127).unsqueeze(-1)).to(torch.bfloat16) for x, s in
+                ((k, scales["k_scale"]), (v, scales["v_scale"])))
+        scales = {}
+    if bad == "table":
+        table[1, 1:4] = torch.tensor([10 ** 6, -1, 2 ** 31 - 1], dtype=torch.int32)
+    elif bad == "length":
+        lens[1] = 2 ** 31 - 1
+    elif bad == "negative":
+        lens[1] = -2 ** 31
+    elif bad == "queries":
+        max_q = new[0] + new[1]
+        cu[1:] += torch.tensor([0, 2 ** 30, 2 ** 30], dtype=torch.int32, device=DEV)
+    else:
+        cu[2] = 0
+    got = C.cache_attention(q, k, v, table, lens, cu, max_q, window=window, **scales)
+    with pytest.raises(KernelStatusError):
+        check_status()
+    _close(got[:new[0]], want[:new[0]], size[:new[0]])
+    if bad in ("table", "length", "negative"):
+        _close(got[2 * new[0]:], want[2 * new[0]:], size[2 * new[0]:])
+    check_status()
