@@ -36,24 +36,27 @@ def kv_cache_read_fp8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: tor
 
 
 def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
-                    cu_q: Optional[torch.Tensor] = None, max_q: int = 1, scale: Optional[float] = None, window: Optional[int] = None,
+                    cu_q: Optional[torch.Tensor] = None, max_q: Optional[int] = None, scale: Optional[float] = None, window: Optional[int] = None,
                     first_tokens: int = 0, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None,
                     out: Optional[torch.Tensor] = None, splits: int = 0) -> torch.Tensor:
     """Causal attention of the new tokens of every sequence over its pages, which hold them already: q [T, hq, d] -> [T, hq, d].
 
     ``block_table`` [B, pages] and ``seq_lens`` [B] (cached tokens, the new ones among them) say where a sequence's tokens lie;
-    ``cu_q`` [B + 1] where its new tokens lie in ``q``, at most ``max_q`` each (None: one token per sequence, a decode step).  The
-    last new token sits at ``seq_lens - 1``.  With ``window`` a token sees itself, the ``window - 1`` tokens in front of it and the
-    ``first_tokens`` first of the sequence; table entries of pages that none of the new tokens sees are not read.  A token that sees
-    nothing (``seq_lens`` smaller than the new tokens) gets zeros.
+    ``cu_q`` [B + 1] where its new tokens lie in ``q`` (None: one token per sequence, a decode step), at most ``max_q`` each (None: as
+    many as ``q`` has; few tokens run as such where it says so).  A sequence with more is refused, on the GPU through the status word
+    and with its rows not written.  The last new token sits at ``seq_lens - 1``.  With ``window`` a token sees itself, the
+    ``window - 1`` tokens in front of it and the ``first_tokens`` first of the sequence; table entries of pages that none of the new
+    tokens sees are not read.  A token that sees nothing (``seq_lens`` smaller than the new tokens) gets zeros, and so does one whose
+    every score is below -1e29.
 
     Pages [blocks, block, hk, d] are bf16, or e4m3 codes with ``k_scale`` and ``v_scale`` as ``kv_cache_write_fp8`` leaves them; a page
     holds a multiple of 16 tokens, heads 64 or 128 numbers, and up to 128 query heads share a key head.  What a page holds
-    behind a sequence's end does not matter.  8-bit values of one sequence may differ by up to 2^100 in size: beside larger ones, smaller
-    ones may count as zero for few tokens.  More than 64 (token, query head of a key head) rows a sequence take scratch of 4 hk d bytes for
-    each 8-bit token that the table has room for, or that ``window`` and ``first_tokens`` let the new tokens see: a gigabyte at a time,
-    one sequence at least.  A value that is NaN or infinite may reach all of its sequence's new tokens, those that
-    it is hidden from among them; a key only those that see it.
+    behind a sequence's end does not matter.  A value that is NaN or infinite may reach all of its sequence's new tokens, those that
+    it is hidden from among them; a key only those that see it.  8-bit values of one sequence may differ by up to 2^100 in size:
+    beside larger ones, smaller ones may count as zero for few tokens.
+
+    More than 64 rows (token, query head of a key head) of 8-bit pages take scratch of 4 hk d bytes for each token that the table has
+    room for, or that the new tokens can see with ``window``: about a gigabyte of sequences at a time, one at least.
 
     Rows of ``q`` that belong to no sequence: those of ``out`` are left as they are; without ``out`` they are zero.  ``splits``: ranges
     that the keys of a block of queries are cut in (0: a rule on the sizes); calls with few tokens cut them in a way of their own."""
@@ -61,7 +64,11 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     scale = d ** -0.5 if scale is None else scale
     if window is not None and window <= 0:
         raise ValueError(f"window {window}: at least the token itself is seen")
+    if max_q is None:
+        max_q = 1 if cu_q is None else q.shape[0]
     if q.is_cuda:
         return kernels().cache_attention(q, k_cache, v_cache, block_table, seq_lens, cu_q, max_q, scale, window or 0, first_tokens,
                                          k_scale, v_scale, out, splits, status_word(q.device))
+    if cu_q is not None and cu_q.numel() > 1 and int(cu_q.diff().max()) > max_q:
+        raise ValueError(f"a sequence of {int(cu_q.diff().max())} new tokens: at most {max_q} were announced")
     return ref.cache_attention(q, k_cache, v_cache, block_table, seq_lens, cu_q, scale, window, first_tokens, k_scale, v_scale, out)

@@ -1,10 +1,11 @@
-"""Which prompts may be continued from a cache: what is refused is refused before the sequence has grown."""
+"""Which prompts may be continued from a cache, and how: what is refused is refused before the sequence has grown."""
 import pytest
 import torch
 
 from pisceslx_b200 import YvConfig
 from pisceslx_b200.models import build_model, generation
 from pisceslx_b200.models.cache import YvCacheConfig, YvPagedKVCache
+from pisceslx_b200.ops import cache as C
 from pisceslx_b200.serve.engine import YvEngineConfig, YvInferenceEngine
 
 TOKENS = torch.randint(0, 300, (80,), generator=torch.Generator().manual_seed(5)).tolist()
@@ -87,3 +88,12 @@ def test_routes_that_are_kept_from_call_to_call_are_not_those_of_another_portion
     model = _model(moe_gate_type="research", extra={"path_moe_stage_size": 2})
     assert model.model.layers[-1].mlp.router.path_stage_size == 2 and not model.supports_portions
     assert _model(moe_gate_type="research").supports_portions
+
+
+def test_more_new_tokens_than_announced_are_refused():
+    q, page = torch.randn(5, 2, 64), torch.randn(1, 16, 1, 64)
+    args = (q, page, page, torch.zeros(2, 1, dtype=torch.int32), torch.tensor([9, 7], dtype=torch.int32), torch.tensor([0, 3, 5], dtype=torch.int32))
+    want = C.cache_attention(*args, 3)
+    assert torch.equal(C.cache_attention(*args), want) and torch.equal(C.cache_attention(*args, max_q=5), want)
+    with pytest.raises(ValueError, match="new tokens"):
+        C.cache_attention(*args, max_q=2)

@@ -211,3 +211,14 @@ def test_what_is_out_of_range_is_reported_and_disturbs_no_other_sequence(bad, ne
     if bad in ("table", "length", "negative"):
         _close(got[2 * new[0]:], want[2 * new[0]:], size[2 * new[0]:])
     check_status()
+
+
+@pytest.mark.parametrize("news", [[3, 1], [40, 7]])
+def test_the_largest_number_of_new_tokens_need_not_be_given(news):
+    args, scales, dense = _case("even", news, [200, 90], 8, 2, 64, 64)
+    got = C.cache_attention(*args[:6], **scales)
+    check_status()
+    _close(got, *_oracle(args[0], dense, news, None, 0))
+    C.cache_attention(*args[:6], max(news) - 1, **scales)
+    with pytest.raises(KernelStatusError):
+        check_status()
