@@ -17,7 +17,7 @@ from typing import Any, Callable, Deque, Dict, Iterator, List, Optional
 
 import torch
 
-from ..models.cache import YvPagedKVCache, cache_for_model
+from ..models.cache import RELEASED, YvPagedKVCache, cache_for_model
 from ..models.generation import YvSampler, YvSamplingConfig, _decode_step, _prefill, to_device
 from ..models.tokenizer import YvTokenizer
 
@@ -134,15 +134,32 @@ class YvInferenceEngine:
     # ---- admission control ---------------------------------------------------------------------------
     def _worst_case_blocks(self, req: YvRequest) -> int:
         remaining = max(req.max_new_tokens - len(req.output_ids), 0)
-        total = len(req.prompt_ids) + len(req.output_ids) + remaining
-        return (total + self.cfg.block_size - 1) // self.cfg.block_size
+        context = len(req.prompt_ids) + len(req.output_ids)
+        return min(-(-(context + remaining) // self.cfg.block_size), self._most_held(context))
+
+    def _most_held(self, context: int) -> int:
+        """Pages that a sequence holds at most, whatever its length, when its ``context`` tokens run as prompt: pages out of every
+        layer's reach have been given back before new ones are taken (``YvPagedKVCache.release_passed``, which keeps those of
+        the first tokens and one of slack)."""
+        bs, cache = self.cfg.block_size, self.cache
+        if cache.reach is None:
+            return cache.cfg.num_blocks + 1
+        size = self._portion() or context
+        kept = -(-cache.cfg.first_tokens // bs)
+        step = size if context > size else 1                       # tokens that are appended to a started sequence at once
+        return max(-(-min(size, context) // bs), kept + 2 - (-(step + cache.reach - 1) // bs))
+
+    def _portion(self) -> int:
+        """Tokens of a prompt that run at once (0 = all)."""
+        return self.cfg.prefill_portion if getattr(self.model, "supports_portions", False) and self.cache.continues else 0
 
     def _owed_blocks(self) -> int:
         """Blocks that running requests may still take: their reservation minus what they already hold.  Running
         sequences allocate lazily (one block every ``block_size`` tokens), so free blocks alone overstate the room."""
         owed = 0
         for rid, need in self._reserved.items():
-            owed += max(need - len(self.cache.tables.get(rid, ())), 0)
+            table = self.cache.tables.get(rid, ())
+            owed += max(need - (len(table) if self.cache.reach is None else sum(b != RELEASED for b in table)), 0)
         return owed
 
     def _preempt_youngest(self) -> bool:
@@ -179,8 +196,7 @@ class YvInferenceEngine:
         if len(tokens) == 1 and self.cache.lengths[seq_id] > 0:
             logits = self.graph.step(list(tokens), [seq_id])
             return logits[[0] * len(want)] if want else None
-        size = self.cfg.prefill_portion if getattr(self.model, "supports_portions", False) and self.cache.continues else 0
-        size = size or len(tokens)
+        size = self._portion() or len(tokens)
         order = sorted(set(want))
         parts = []
         for lo in range(0, len(tokens), size):
@@ -201,7 +217,8 @@ class YvInferenceEngine:
         while self.waiting and len(self.running) < self.cfg.max_num_seqs:
             req = self.waiting[0]
             now = (len(req.prompt_ids) + len(req.output_ids) + self.cfg.block_size) // self.cfg.block_size
-            need = max(self._worst_case_blocks(req), now)  # ``now``: prefill plus the first decoded token
+            # ``now``: prefill plus the first decoded token
+            need = max(self._worst_case_blocks(req), min(now, self._most_held(len(req.prompt_ids) + len(req.output_ids))))
             if need > self.cache.alloc.available() - self._owed_blocks():
                 if not self.running:
                     self.waiting.popleft()
