@@ -217,21 +217,27 @@ class YvPagedKVCache:
                 "k_scale": [t.cpu() for t in self.k_scale], "v_scale": [t.cpu() for t in self.v_scale]}
 
     def load_state(self, st: Dict[str, object]) -> None:
-        self.tables = {int(k): list(v) for k, v in st["tables"].items()}      # type: ignore[union-attr]
-        self.lengths = {int(k): int(v) for k, v in st["lengths"].items()}     # type: ignore[union-attr]
-        used = {b for t in self.tables.values() for b in t if b != RELEASED}
-        self.alloc = YvBlockAllocator(self.cfg.num_blocks)
-        self.alloc.free = [b for b in range(self.cfg.num_blocks - 1, -1, -1) if b not in used]
-        self.alloc.refs = {b: sum(b in t for t in self.tables.values()) for b in used}
+        pairs = []
         for mine, saved in ((self.k, st["k"]), (self.v, st["v"]), (self.k_scale, st.get("k_scale", [])),
                             (self.v_scale, st.get("v_scale", []))):
             if len(mine) != len(saved):                                        # type: ignore[arg-type]
                 raise ValueError("the saved cache holds its keys and values in another form")
             for t, src in zip(mine, saved):                                    # type: ignore[arg-type]
                 if t is not None:
+                    if src is None or t.shape != src.shape:
+                        raise ValueError(f"saved pages of {None if src is None else tuple(src.shape)} for {tuple(t.shape)}")
                     if t.dtype != src.dtype and torch.float8_e4m3fn in (t.dtype, src.dtype):
                         raise ValueError(f"a saved cache of {src.dtype} for one of {t.dtype}")
-                    t.copy_(src)
+                    pairs.append((t, src))
+        # nothing has been touched so far
+        self.tables = {int(k): list(v) for k, v in st["tables"].items()}      # type: ignore[union-attr]
+        self.lengths = {int(k): int(v) for k, v in st["lengths"].items()}     # type: ignore[union-attr]
+        used = {b for t in self.tables.values() for b in t if b != RELEASED}
+        self.alloc = YvBlockAllocator(self.cfg.num_blocks)
+        self.alloc.free = [b for b in range(self.cfg.num_blocks - 1, -1, -1) if b not in used]
+        self.alloc.refs = {b: sum(b in t for t in self.tables.values()) for b in used}
+        for t, src in pairs:
+            t.copy_(src)
 
 
 class YvPagedLayeredCache(YvPagedKVCache):

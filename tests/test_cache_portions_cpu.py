@@ -97,3 +97,35 @@ def test_more_new_tokens_than_announced_are_refused():
     assert torch.equal(C.cache_attention(*args), want) and torch.equal(C.cache_attention(*args, max_q=5), want)
     with pytest.raises(ValueError, match="new tokens"):
         C.cache_attention(*args, max_q=2)
+
+
+def test_a_saved_cache_of_another_form_leaves_the_cache_as_it_was(model):
+    def filled(**kw):
+        cache = _cache(model, **kw)
+        cache.add_sequence(1)
+        _run(model, cache, TOKENS[:40])
+        return cache
+    plain, small = filled(), YvPagedKVCache(2, model.cfg.n_kv_head, model.cfg.head_dim, YvCacheConfig(
+        block_size=16, num_blocks=16, dtype=torch.float8_e4m3fn), torch.device("cpu"))
+    small.add_sequence(7)
+    _run_in(model, small, 7, TOKENS[:20])
+    one_layer = {k: v[:1] if k in ("k", "v") else v for k, v in plain.state().items()}
+    other_pages = {k: [t[:, :8] for t in v] if k in ("k", "v") else v for k, v in plain.state().items()}
+    for cache, states in ((plain, (small.state(), one_layer, other_pages)), (small, (plain.state(), other_pages))):
+        before = cache.state()
+        free, refs = list(cache.alloc.free), dict(cache.alloc.refs)
+        before = {k: [t.clone() for t in v] if isinstance(v, list) else v for k, v in before.items()}
+        for state in states:
+            with pytest.raises(ValueError):
+                cache.load_state(state)
+        after = cache.state()
+        assert (after["tables"], after["lengths"], cache.alloc.free, cache.alloc.refs) == (before["tables"], before["lengths"], free, refs)
+        for name in ("k", "v", "k_scale", "v_scale"):
+            assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(before[name], after[name]))
+    copy = _cache(model)
+    copy.load_state(plain.state())
+    assert torch.equal(copy.k[1], plain.k[1]) and copy.lengths == {1: 40}
+
+
+def _run_in(model, cache, seq, tokens):
+    return generation._prefill(model, torch.tensor([tokens]), cache, [seq])
