@@ -19,8 +19,9 @@ namespace {
 constexpr int kRowsThreads = 256;
 
 // One group of d / 8 lanes per row: 16 bytes in, 8 bytes of codes out, a byte by the first lane.
-// Bound by bytes: 8191 tokens of 8 heads of 128 (50 MB) take 19 us from a cold cache, a copy of as many bytes 22.6; two or four rows
-// a group, loaded ahead, 20.5.
+// 8191 tokens of 8 heads of 128 (50 MB) take 17.5 us from a cold cache in a captured run of calls, a copy of as many bytes 18.1 in
+// the same way (7.8 at the rate of a copy of gigabytes); 18.8 call by
+// call.  Two or four rows a group, loaded ahead, 20.5 for 19.
 template <int D, bool CHAIN>
 __global__ void __launch_bounds__(kRowsThreads) cache_write_fp8_kernel(const CacheRowsArgs a) {
   constexpr int kLanes = D / 8;
@@ -221,7 +222,7 @@ int widened_room(const CacheAttnArgs& a) {
 }
 
 // Rows (token, head of a group) that the kernel for few tokens holds, 0 where cache_attn_kernel takes the call.  That one would
-// have to widen 8-bit pages first: 16 sequences of 8192 tokens with 16 new ones, 4 heads a group: 115 us here, 17 new ones there 211.
+// have to widen 8-bit pages first: 16 sequences of 8192 tokens with 16 new ones, 4 heads a group: 137 us here, 17 new ones there 250.
 // Pages in bf16 it reads as they are, and its 128 rows cost no more than the keys' bytes.  It is the slower one where its key
 // ranges are uneven or too short, that is for up to 16 rows and many sequences (64 of up to 3000 tokens, 8 key heads, one new one:
 // 137 us against 121 here; 16 of 8192: 98 and 98) or for little in all (one of 2048 tokens: 16.4 and 13.8; of 8192: 29.6 and 28.7;

@@ -18,12 +18,14 @@
 //   warp 11     gives its registers away
 // TMEM columns: [0,128) S0/P0, [128,256) S1/P1, [256,256+D) O0, [384,384+D) O1.
 //
-// 32 query heads over 8 of 128: 512 tokens of 16384 157 us (863 TFLOP/s; 82 at the measured peak), 4096 of 32768 over 8-bit pages
-// 2022 us (1020 TFLOP/s; 1257).  A step, a key tile for both query tiles, takes 3700 cycles where its products take 2048: the
-// softmax of a half (2000) and the products of that half (1000, and as much behind the other's) follow one another, and both halves
-// with their scores, weights and sums fill the tensor memory, so that there is no room for a half's next scores.  In parts of 64 keys
-// there is, but their products read the query tile twice as often (180 us).  Weights handed over in two portions: 161 us.  An item
-// costs 6 us to begin and to end besides.
+// 32 query heads over 8 of 128: 512 tokens of 16384 158 us (856 TFLOP/s; 82 at the measured peak), 4096 of 32768 over 8-bit pages
+// 2035 us (1010 TFLOP/s; 1254).  The kernel for prompts (attention_fwd.cuh), whose pipeline this is, takes a prompt without a prefix
+// 8 to 9 % faster (16384 tokens 1926 us for 2085, 4096 127 for 140): pages in boxes, slots looked up, keys cleared.  The rest of the
+// distance to the peak both have: a step, a key tile for both query tiles, takes 3700 cycles here where its products take 2048, since
+// the softmax of a half (2000) and its products (1000, and as much behind the other's) follow one another.  Scores of a half's next
+// tile ahead of that take tensor memory that only parts of 64 keys leave free, and then its products read the query tile twice as
+// often (180 us).  Weights handed over in two portions: 161 us.  An item costs 6 us to begin and to end besides, and a short call is
+// uneven: 128 of 148 SMs have work in the first of these.
 //
 // What a page holds past the end of a sequence, or in front of everything that the block sees, may be anything: its scores are
 // masked and its values cleared (a zero weight times NaN is NaN).

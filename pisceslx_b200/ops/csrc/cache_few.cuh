@@ -34,9 +34,9 @@
 // unrolled, in registers, what is done once an item cost more than its tiles (18 sequences of 2048 tokens, 16 new ones: 270 us;
 // 16 of them take 59 in loops).
 //
-// 8-bit pages, 32 query heads over 8 of 128: 64 sequences of 2048 to 4096 tokens, a new one each, 89 us (4.7 TB/s of codes, 71 % of a
-// copy's rate; a tile takes an SM 0.85 us, its bytes 0.75); 8 of up to 8192 with 5 new ones 51 us (17.8 for the bytes; a tile 1.4 us,
-// 1.75 with 16 new ones).  Of each call 12 us or so are the beginning, the last parts and the join.  Scores of a piece's next tile
+// 8-bit pages, 32 query heads over 8 of 128: 64 sequences of 2048 to 4096 tokens, a new one each, 95 us (4.2 TB/s of codes, 64 % of the
+// measured copy rate; a tile takes an SM 0.85 us, its bytes 0.75); 8 of up to 8192 with 5 new ones 53 us (15.5 for the bytes; a tile 1.4
+// us, 1.75 with 16 new ones).  Of each call 12 us or so are the beginning, the last parts and the join.  Scores of a piece's next tile
 // ahead of a product with the values, in a second buffer, made it slower (one new token 1.11 us a tile for 0.83, four 1.41 for
 // 1.04), and so did, from 32 rows on, loads of the next 16 rows' scores in front of the weights of these (2 to 5 %).
 #pragma once
