@@ -53,7 +53,8 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     holds a multiple of 16 tokens, heads 64 or 128 numbers, and up to 128 query heads share a key head.  What a page holds
     behind a sequence's end does not matter.  A value that is NaN or infinite may reach all of its sequence's new tokens, those that
     it is hidden from among them; a key only those that see it.  8-bit values of one sequence may differ by up to 2^100 in size:
-    beside larger ones, smaller ones may count as zero for few tokens.
+    beside larger ones, smaller ones may count as zero for few tokens.  Over 8-bit pages a few tokens' queries are held to 2^-22 of the
+    largest of their row's numbers (those above 2^-14 of it exactly).
 
     More than 64 rows (token, query head of a key head) of 8-bit pages take scratch of 4 hk d bytes for each token that the table has
     room for, or that the new tokens can see with ``window``: about a gigabyte of sequences at a time, one at least.

@@ -84,8 +84,8 @@ def _oracle(q, dense, new, window, first):
 
 def _close(got, want, size):
     """Weights are rounded to 8 bits at worst (2^-8 of each), the result too (2^-8 of it).  The rest is within 2^-10 of what the weights
-    make of the values: 2^x to 1e-4, and fp16 weights, which are off by 2^-29 of the largest row beside others within 2^6 of it: of
-    2100 keys 2^-12 of the largest."""
+    make of the values: 2^x to 1e-4, and fp16 weights, which are off by 2^-29 of the largest row beside others within 2^7 of it, 2^-22
+    of what counts most for each key: 2^-12 where 1000 keys are all rounded alike (2100 rounded at random: 2^-16)."""
     top = size.amax(-1, keepdim=True)                 # codes of one row differ in size: what a weight is off by is relative to the row
     bad = (got.double() - want).abs() > (2.0 ** -8 + 2.0 ** -10) * size + 2.0 ** -12 * top + 2.0 ** -8 * want.abs()
     assert torch.isfinite(got).all() and not bad.any(), (int(bad.sum()), bad.numel(), float(((got.double() - want).abs() / top).max()))
